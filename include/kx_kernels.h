@@ -246,6 +246,74 @@ KERNIX_API int kx_conv_f32_ws(const float* x, const float* w_hi, const float* w_
 KERNIX_API int kx_attention(const float* q, int ldq, const float* k, int ldk, const float* v, int ldv, float* ctx, int ldc, int B,
                  int Rq, int S, int H, int dk, int dv, int causal, int* status, void* stream);
 
+/* ---- paged key-value cache: its pages, the attention of one new token over it, windowed prompt attention ----
+ * Extensions next to the ATTENTION step's kx_attention (kernix_attention_run :1005-1048); the reference has no cache.
+ *
+ * A kx_kv describes a cache in device memory that the caller owns; the struct itself is host memory, read during the
+ * call only. K and V live in pools of pages: page p of layer l holds `page` tokens of every key-value head,
+ *   K: k + l * k_layer + p * k_page (elements), heads x page x dk, dense;  V: likewise with dv.
+ * Sequence slot s holds lens[s] tokens on the pages table[s * max_pages + j], j < ceil(lens[s] / page); the entries
+ * behind them are -1. refs[p] counts the table entries that name page p; 0 means free. The tables serve every layer.
+ * An empty cache has lens = 0, refs = 0, table = -1; the entry points below keep these consistent.
+ * Requirements, else -1: page a power of two up to 1024; dk * size and dv * size multiples of 16 bytes, dk, dv <= 1024;
+ * k, v and all strides * size multiples of 16 bytes; pages (and layers) that do not overlap;
+ * max_pages * page < 2^31; heads * page * dk and heads * page * dv <= 2^28. Calls that change a cache are ordered on one stream (or by events) with those that use it.
+ *
+ * Requests live in device memory, so a kernel checks them: what it refuses it leaves out, memory-safely, and ORs a bit
+ * into *status (device word, may be NULL; never cleared here): KX_STATUS_NO_PAGES, too few free pages or a full table
+ * row; KX_STATUS_BAD_REQUEST, a slot, length or page id out of range, or a slot that may not be used so. */
+#define KX_KV_F32 0
+#define KX_KV_F16 1
+#define KX_KV_BF16 2
+#define KX_STATUS_NO_PAGES 2
+#define KX_STATUS_BAD_REQUEST 4
+typedef struct {
+    int type;                            /* element type of the pools: KX_KV_F32, KX_KV_F16 or KX_KV_BF16 */
+    int layers, n_pages, page, heads, dk, dv;
+    int n_seqs, max_pages;               /* slots; pages per slot at most */
+    void* k;
+    void* v;
+    long k_page, k_layer;                /* elements from one page to the next, from one layer to the next */
+    long v_page, v_layer;
+    int32_t* table;                      /* n_seqs x max_pages */
+    int32_t* lens;                       /* n_seqs */
+    int32_t* refs;                       /* n_pages */
+} kx_kv;
+
+/* bytes of device workspace (16-byte aligned) for extend, fork and compact on this cache; its contents need no
+ * preparation and carry nothing from call to call, so calls may share one workspace unless they overlap on the GPU
+ * (calls on different streams and concurrently replayed graphs each need their own). 0 if the description is invalid. */
+KERNIX_API size_t kx_kv_ws(const kx_kv* c);
+
+/* Room for want[s] more tokens in every slot s (want: n_seqs words; <= 0 asks for nothing): pages are taken for them, lens[s] += want[s]
+ * and granted[s] = want[s]; a refused slot is left as it was with granted[s] = 0 (want and granted may be the same
+ * array). Slots are served in order and pages taken lowest id first; once a slot's need exceeds what is free, it and
+ * every later slot that needs a page is refused. The new tokens are then written by kx_kv_append, layer by layer. */
+KERNIX_API int kx_kv_extend(const kx_kv* c, const int32_t* want, int32_t* granted, void* ws, size_t ws_bytes, int* status,
+                            void* stream);
+
+/* The last count[s] tokens of every slot s (positions lens[s] - count[s] .. lens[s] - 1) of one layer from fp32 rows
+ * s * rows + i, i < count[s] (<= rows; <= 0: none): heads * dk floats of k at leading dimension ldk, heads * dv of v at
+ * ldv, rounded to the cache's type (to nearest even). Rows i >= count[s] are not read. k and v must not overlap the pools. */
+KERNIX_API int kx_kv_append(const kx_kv* c, int layer, const float* k, int ldk, const float* v, int ldv, const int32_t* count,
+                            int rows, int* status, void* stream);
+
+/* dst[i] becomes a copy of the sequence in src[i], i < n <= n_seqs: full pages are shared (refs + 1), a partly filled
+ * last page is copied to a fresh page (every layer; lowest free ids, in order of i), so that either may grow. All pairs
+ * see the state before the call. Refused: dst[i] not empty (lens != 0), equal to src[i] or already named by an earlier
+ * pair, slots or lengths out of range; and, once pages run out, each pair from there on that needs one. A pair with
+ * dst[i] < 0 is skipped. A parent's page id out of range is passed on as -1 (and reported). */
+KERNIX_API int kx_kv_fork(const kx_kv* c, const int32_t* src, const int32_t* dst, int n, void* ws, size_t ws_bytes, int* status,
+                          void* stream);
+
+/* The slots seqs[i], i < n, become empty; each of their pages loses a reference. Slots < 0 are skipped, a slot may be
+ * named twice. */
+KERNIX_API int kx_kv_free(const kx_kv* c, const int32_t* seqs, int n, int* status, void* stream);
+
+/* Moves pages so that the live ones (refs != 0) are the pages 0 .. *n_live - 1: the r-th free page below n_live takes
+ * the contents (every layer), references and table entries of the r-th live page from n_live on. n_live: device word. */
+KERNIX_API int kx_kv_compact(const kx_kv* c, int32_t* n_live, void* ws, size_t ws_bytes, void* stream);
+
 /* y = max(a*x + b, 0), fused multiply-add then max (src/kernix_metal.m:331-338; include/kernix.h:990) */
 KERNIX_API int kx_fma_relu(const float* a, const float* x, const float* b, float* y, size_t n, void* stream);
 

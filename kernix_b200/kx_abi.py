@@ -44,6 +44,11 @@ SIGNATURES = {
     "kx_conv_f32": [_vp, _vp, _vp, _i, _vp, _vp] + [_i] * 16 + [_i, _f, _vp, _vp],
     "kx_conv_f32_ws": [_vp, _vp, _vp, _i, _vp, _vp] + [_i] * 16 + [_i, _f, _vp, _sz, _vp, _vp],
     "kx_attention": [_vp, _i, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp],
+    "kx_kv_extend": [_vp, _vp, _vp, _vp, _sz, _vp, _vp],
+    "kx_kv_append": [_vp, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _vp],
+    "kx_kv_fork": [_vp, _vp, _vp, _i, _vp, _sz, _vp, _vp],
+    "kx_kv_free": [_vp, _vp, _i, _vp, _vp],
+    "kx_kv_compact": [_vp, _vp, _vp, _sz, _vp],
     "kx_fma_relu": [_vp, _vp, _vp, _vp, _sz, _vp],
     "kx_unshard_cols": [_vp, _i, _l, _i, _vp, _i, _vp],
     "kx_rnn_step": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp],
@@ -54,6 +59,19 @@ SIGNATURES = {
     "kx_knx_inspect": [ctypes.c_char_p, ctypes.POINTER(_l), ctypes.POINTER(_i), ctypes.POINTER(_i), ctypes.POINTER(_i), _i,
                        ctypes.c_char_p, _i],
 }
+
+# entry points that return a number of bytes
+SIZES = {
+    "kx_kv_ws": [_vp],
+}
+
+
+class KvCache(ctypes.Structure):
+    """kx_kv (include/kx_kernels.h): a paged key-value cache. Pass ctypes.byref(cache)."""
+    _fields_ = ([(n, _i) for n in ("type", "layers", "n_pages", "page", "heads", "dk", "dv", "n_seqs", "max_pages")]
+                + [("k", _vp), ("v", _vp)] + [(n, _l) for n in ("k_page", "k_layer", "v_page", "v_layer")]
+                + [("table", _vp), ("lens", _vp), ("refs", _vp)])
+
 
 _done = False
 
@@ -66,6 +84,10 @@ def lib():
             fn = getattr(L, name)
             fn.argtypes = args
             fn.restype = ctypes.c_int
+        for name, args in SIZES.items():
+            fn = getattr(L, name)
+            fn.argtypes = args
+            fn.restype = _sz
         _done = True
     return L
 
