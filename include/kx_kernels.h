@@ -314,6 +314,20 @@ KERNIX_API int kx_kv_free(const kx_kv* c, const int32_t* seqs, int n, int* statu
  * the contents (every layer), references and table entries of the r-th live page from n_live on. n_live: device word. */
 KERNIX_API int kx_kv_compact(const kx_kv* c, int32_t* n_live, void* ws, size_t ws_bytes, void* stream);
 
+/* Attention of one new token per row over the cache (scaled dot products as kx_attention, keys and values read from
+ * their pages): row i, i < n, is the last token (position lens - 1, appended before) of slot seqs[i] (seqs NULL: slot i),
+ * its H query heads in q + i * ldq (H * dk floats); query head h reads key-value head h / (H / heads). It sees key j
+ * when window <= 0, or j > lens - 1 - window, or j < sinks. ctx + i * ldc receives H * dv floats. scale 0 means
+ * 1/sqrt(dk). A row with seqs[i] < 0 is left as it was, one whose slot holds no tokens becomes 0, and one whose slot,
+ * length or (visible) pages are out of range becomes NaN and is reported. H a multiple of heads, dk, dv <= 128. q and ctx
+ * must not overlap each other or the cache. ws: kx_attention_paged_ws bytes of device workspace (0: the arguments are
+ * invalid), to be shared under kx_kv_ws's rules. Results do not depend on timing: the same call on the same contents
+ * gives the same bits. */
+KERNIX_API size_t kx_attention_paged_ws(const kx_kv* c, int H, int n);
+KERNIX_API int kx_attention_paged(const kx_kv* c, int layer, const float* q, int ldq, int H, const int32_t* seqs, int n, int window,
+                                  int sinks, float scale, float* ctx, int ldc, void* ws, size_t ws_bytes, int* status,
+                                  void* stream);
+
 /* y = max(a*x + b, 0), fused multiply-add then max (src/kernix_metal.m:331-338; include/kernix.h:990) */
 KERNIX_API int kx_fma_relu(const float* a, const float* x, const float* b, float* y, size_t n, void* stream);
 

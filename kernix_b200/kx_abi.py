@@ -49,6 +49,7 @@ SIGNATURES = {
     "kx_kv_fork": [_vp, _vp, _vp, _i, _vp, _sz, _vp, _vp],
     "kx_kv_free": [_vp, _vp, _i, _vp, _vp],
     "kx_kv_compact": [_vp, _vp, _vp, _sz, _vp],
+    "kx_attention_paged": [_vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _f, _vp, _i, _vp, _sz, _vp, _vp],
     "kx_fma_relu": [_vp, _vp, _vp, _vp, _sz, _vp],
     "kx_unshard_cols": [_vp, _i, _l, _i, _vp, _i, _vp],
     "kx_rnn_step": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp],
@@ -63,6 +64,7 @@ SIGNATURES = {
 # entry points that return a number of bytes
 SIZES = {
     "kx_kv_ws": [_vp],
+    "kx_attention_paged_ws": [_vp, _i, _i],
 }
 
 

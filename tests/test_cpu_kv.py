@@ -62,3 +62,21 @@ def test_nothing_to_do_launches_nothing(kx):
     assert L.kx_kv_free(ref(c), None, 0, None, None) == 0
     assert L.kx_kv_fork(ref(c), None, None, 0, p, n, None, None) == 0
     assert L.kx_kv_append(ref(c), 0, None, 0, None, 0, None, 0, None, None) == 0
+
+
+def test_paged_attention_refuses_bad_arguments(kx):
+    c, L = fake(kx), kx.lib()
+    p, n = 0x60000, kx.lib().kx_attention_paged_ws(ref(c), 4, 2)
+    assert n > 0
+
+    def call(c=c, layer=0, q=p, ldq=256, H=4, seqs=None, n_rows=2, window=0, sinks=0, scale=0.0, ctx=p, ldc=256, ws=p, nbytes=n):
+        return L.kx_attention_paged(ref(c), layer, q, ldq, H, seqs, n_rows, window, sinks, scale, ctx, ldc, ws, nbytes, None, None)
+
+    for kw in [dict(layer=2), dict(layer=-1), dict(q=None), dict(ldq=255), dict(H=3), dict(H=0), dict(n_rows=5), dict(n_rows=-1),
+               dict(sinks=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(ctx=None), dict(ldc=255), dict(ws=None),
+               dict(ws=p + 4), dict(nbytes=n - 1)]:
+        assert call(**kw) == -1, kw
+    for kw in BAD + [dict(dk=136, k_page=2 * 16 * 136, k_layer=10 * 2 * 16 * 136)]:
+        bad = fake(kx, **kw)
+        assert L.kx_attention_paged_ws(ref(bad), 4, 2) == 0 and call(c=bad) == -1, kw
+    assert call(n_rows=0) == 0
