@@ -18,9 +18,11 @@
 //     a ring of its own in shared memory: deep prefetch without registers and without barriers. The order of the
 //     reduction axis inside a product is free, so a lane's 16 contiguous bytes serve as they lie; masked keys are
 //     zero-filled and never read.
-//   * Work split: the steps of all rows and heads form one line, cut into equal ranges, one per CTA (two CTAs per SM);
-//     a range may cover several short sequences or a part of a long one. A head whose steps lie in several ranges is
-//     joined by a second launch (programmatic dependent) in the order of the ranges: nothing depends on timing.
+//   * Work split: the steps of all rows and heads form one line, cut into equal ranges, one per warp (eight warps per
+//     SM); a range may cover several short sequences or a part of a long one. A head whose steps lie in several ranges
+//     is joined by a second launch (programmatic dependent) in the order of the ranges: nothing depends on timing.
+//     (One range per CTA, its warps meeting in shared memory at every unit, took 73 us where this takes XX: a CTA
+//     that got many short sequences paid the meeting for each.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -48,8 +50,9 @@ constexpr unsigned FULL = 0xFFFFFFFFu;
 constexpr int PG_WARPS = 4, PG_THREADS = PG_WARPS * 32;
 constexpr int PG_STAGES = 3;
 constexpr int PG_HEADS = 8;       // query heads per tile
-constexpr int PG_MAX_CTAS = 512;  // of a split launch: sizes the workspace
-constexpr int PG_MIN_STEPS = 4 * PG_WARPS;  // a CTA's range is at least this many steps: the join costs as much as a few
+constexpr int PG_MAX_WARPS = 1280;  // of a launch over the line: sizes the workspace
+constexpr int PG_MIN_STEPS = 4;     // a warp's range is at least this many steps: a part more costs as much as a few
+constexpr int PG_UNIT_STEPS = 24;   // a unit of at most this many steps is one CTA's
 constexpr int PG_DMAX = 128;
 
 struct PagedArgs {
@@ -61,15 +64,15 @@ struct PagedArgs {
     char* ws;
     int* status;
     int n, H, G, chunks, per_chunk;  // query heads per key-value head, tiles of heads per key-value head, heads per tile
-    int ldq, ldc, window, sinks, grid;
+    int ldq, ldc, window, sinks;
     float scale2;
-    bool vecq;
+    bool vecq, vecc;
 };
 
-// what a CTA's range begins with: written by the main launch, read by the join
+// what a warp's range begins with: written by the main launch, read by the join
 struct PagedDesc {
     long long first;  // position of the unit's first step on the line
-    long long per;    // steps per CTA
+    long long per;    // steps per warp
     int row, unit, steps, pad;
 };
 
@@ -115,19 +118,19 @@ __device__ __forceinline__ uint4 lds16(uint32_t a) {
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]));
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]));
 }
 __device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]));
 }
 
 // two fp32 values as PARTS pairs of the 16-bit type, the value = the sum of its parts up to the last one's rounding
@@ -149,11 +152,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, float* ra, float* rb
     }
     return w;
 }
+// v = hi + rest with 11 bits in hi (cut off, two instructions; the tensor core cuts rest to 11 bits: 2^-21 of v is lost)
 __device__ __forceinline__ uint32_t tf32_of(float v, float* rest) {
-    float hi, lo;
-    kx::tf32_split(v, hi, lo);
-    *rest = lo;
-    return __float_as_uint(hi);
+    const uint32_t hi = __float_as_uint(v) & 0xFFFFE000u;
+    *rest = v - __uint_as_float(hi);
+    return hi;
 }
 
 template <int TYPE, int D>
@@ -173,172 +176,222 @@ struct Shape {
     static_assert(PG_STAGES * STAGE >= PG_HEADS * D * 4, "a warp's ring holds its partial output");
 };
 
-// One unit's steps [i0, i1) (of sp.steps) by the whole CTA. UNSPLIT results go to ctx, others to `part`.
+// where a warp is on the line: step i of unit `unit` (key-value head x tile of heads) of row `row`
 template <int TYPE, int D>
-__device__ void paged_piece(const PagedArgs& A, uint8_t* smem, float (&red)[PG_WARPS][PG_HEADS][2], int row, int slot, const Span& sp,
-                            int unit, int i0, int i1, float* part) {
+struct Cursor {
     using S = Shape<TYPE, D>;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int kvh = unit / A.chunks, head0 = kvh * A.G + (unit - kvh * A.chunks) * A.per_chunk;
-    const int heads = min(A.per_chunk, (kvh + 1) * A.G - head0);
-    const int nck = A.c.dk / S::EPC, ncv = A.c.dv / S::EPC, shift = 31 - __clz(A.c.page);
-    const int32_t* table = A.c.table + static_cast<long>(slot) * A.c.max_pages;
-    constexpr long SZ = 16 / S::EPC;
-    const char* kb = A.k + static_cast<long>(kvh) * A.c.page * A.c.dk * SZ;
-    const char* vb = A.v + static_cast<long>(kvh) * A.c.page * A.c.dv * SZ;
-    const uint32_t ring = kx::smem_u32(smem) + warp * (PG_STAGES * S::STAGE) + lane * 16;
-    bool bad = sp.bad;
+    Span sp;
+    int row, slot, unit, i;
 
-    const auto first_key = [&](int i) { return (i < sp.na ? i : i - sp.na + sp.b0) * S::KS; };
-    const auto visible = [&](int j) { return j < sp.len && (j < sp.s0 || j >= sp.w0); };
-    // page of key first_key(i) + lane % KS, one step ahead of its use
-    const auto page_of = [&](int i) {
-        const int j = first_key(i) + (lane & (S::KS - 1));
-        return i < i1 && visible(j) ? __ldg(table + (j >> shift)) : 0;
-    };
-    const auto issue = [&](int i, int pid, int stage) {
-        if (i < i1) {
-            const int base = first_key(i);
-            if (pid < 0 || pid >= A.c.n_pages) {
-                bad = true;  // this key's page is not there: the row becomes NaN, nothing is read
-                pid = -1;
-            }
-            const uint32_t dst = ring + stage * S::STAGE;
+    __device__ __forceinline__ void seek_row(const PagedArgs& A, int r) {  // rows that are left alone have no steps
+        do {
+            row = r++;
+            sp = span_of<S::KS>(A, row, &slot);
+        } while (sp.steps == 0);
+    }
+    // the next step; false: it is another unit's. Not called at the end of the line.
+    __device__ __forceinline__ bool next(const PagedArgs& A, int units) {
+        if (++i < sp.steps) return true;
+        i = 0;
+        if (++unit == units) {
+            unit = 0;
+            seek_row(A, row + 1);
+        }
+        return false;
+    }
+    __device__ __forceinline__ int first_key() const { return (i < sp.na ? i : i - sp.na + sp.b0) * S::KS; }
+    // every key of the step is seen
+    __device__ __forceinline__ bool whole() const {
+        const int j = first_key();
+        return j + S::KS <= sp.len && (j >= sp.w0 || j + S::KS <= sp.s0);
+    }
+    __device__ __forceinline__ bool visible(int j) const { return j < sp.len && (j < sp.s0 || j >= sp.w0); }
+};
+
+// The loads of a warp: page ids 32 at a time (one per lane), then every lane the chunks of a step that it will use.
+template <int TYPE, int D>
+struct Feed {
+    using S = Shape<TYPE, D>;
+    static constexpr long SZ = 16 / S::EPC;
+    const int32_t* table;
+    const char *kb, *vb;
+    int ids, base;  // ids: table[base + lane]
+
+    __device__ __forceinline__ void unit(const PagedArgs& A, const Cursor<TYPE, D>& c) {
+        const int kvh = c.unit / A.chunks;
+        table = A.c.table + static_cast<long>(c.slot < A.c.n_seqs ? c.slot : 0) * A.c.max_pages;
+        kb = A.k + static_cast<long>(kvh) * A.c.page * A.c.dk * SZ;
+        vb = A.v + static_cast<long>(kvh) * A.c.page * A.c.dv * SZ;
+        base = -64;
+    }
+    // false: a page that a visible key lies on is not there (its key is then zero-filled, nothing is read)
+    __device__ __forceinline__ bool issue(const PagedArgs& A, const Cursor<TYPE, D>& c, uint32_t dst, int nck, int ncv, int shift) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, first = c.first_key();
+        if ((first >> shift) < base || ((first + S::KS - 1) >> shift) >= base + 32) {
+            base = first >> shift;
+            ids = base + lane <= (c.sp.len - 1) >> shift ? __ldcg(table + base + lane) : 0;
+        }
+        if (A.c.page >= S::KS && c.whole()) {  // one page, every key seen: one base address for K and one for V
+            const int p = __shfl_sync(FULL, ids, (first >> shift) - base);
+            if (p >= 0 && p < A.c.n_pages) {
+                const int slot = first & (A.c.page - 1);
+                const char* ks = kb + p * A.c.k_page * SZ + static_cast<long>((slot + g) * nck + t) * 16;
+                const char* vs = vb + p * A.c.v_page * SZ + static_cast<long>((slot + 2 * t) * ncv + g) * 16;
 #pragma unroll
-            for (int u = 0; u < S::KT; u++) {
-                const int j = base + u * 8 + g, p = __shfl_sync(FULL, pid, u * 8 + g);
-                const bool ok = visible(j) && p >= 0;
-                const char* src = ok ? kb + p * A.c.k_page * SZ + (static_cast<long>(j & (A.c.page - 1)) * nck + t) * 16 : A.k;
+                for (int x = 0; x < S::KCH; x++) {
+                    if (x * 4 >= nck) continue;
+                    const bool in = x * 4 + t < nck;
+                    const char* src = in ? ks + x * 64 : A.k;
 #pragma unroll
-                for (int c = 0; c < S::KCH; c++) {
-                    const bool in = ok && c * 4 + t < nck;
-                    if (c * 4 < nck) cp16(dst + (u * S::KCH + c) * 512, in ? src + c * 64 : A.k, in);
+                    for (int u = 0; u < S::KT; u++) cp16(dst + (u * S::KCH + x) * 512, src + (in ? u * 128 * nck : 0), in);
                 }
-            }
 #pragma unroll
-            for (int u = 0; u < S::VK; u++) {
-                const int x = (u >> 1) * 8 + 2 * t + (u & 1), j = base + x, p = __shfl_sync(FULL, pid, x);
-                const bool ok = visible(j) && p >= 0;
-                const char* src = ok ? vb + p * A.c.v_page * SZ + (static_cast<long>(j & (A.c.page - 1)) * ncv + g) * 16 : A.v;
+                for (int x = 0; x < S::VCH; x++) {
+                    if (x * 8 >= ncv) continue;
+                    const bool in = x * 8 + g < ncv;
+                    const char* src = in ? vs + x * 128 : A.v;
 #pragma unroll
-                for (int c = 0; c < S::VCH; c++) {
-                    const bool in = ok && c * 8 + g < ncv;
-                    if (c * 8 < ncv) cp16(dst + (S::KT * S::KCH + u * S::VCH + c) * 512, in ? src + c * 128 : A.v, in);
+                    for (int u = 0; u < S::VK; u++)
+                        cp16(dst + (S::KT * S::KCH + u * S::VCH + x) * 512, src + (in ? ((u >> 1) * 8 + (u & 1)) * 16 * ncv : 0), in);
                 }
+                return true;
             }
         }
-        cp_commit();
-    };
-
-    // the first stages on their way before q is looked at
-    int pid = page_of(i0 + warp);
+        bool good = true;
 #pragma unroll
-    for (int s = 0; s < PG_STAGES - 1; s++) {
-        const int next = page_of(i0 + warp + (s + 1) * PG_WARPS);
-        issue(i0 + warp + s * PG_WARPS, pid, s);
-        pid = next;
+        for (int u = 0; u < S::KT; u++) {
+            const int j = first + u * 8 + g, p = __shfl_sync(FULL, ids, (j >> shift) - base);
+            const bool see = c.visible(j), ok = see && p >= 0 && p < A.c.n_pages;
+            good = good && (ok || !see);
+            const char* src = ok ? kb + p * A.c.k_page * SZ + (static_cast<long>(j & (A.c.page - 1)) * nck + t) * 16 : A.k;
+#pragma unroll
+            for (int x = 0; x < S::KCH; x++) {
+                const bool in = ok && x * 4 + t < nck;
+                if (x * 4 < nck) cp16(dst + (u * S::KCH + x) * 512, in ? src + x * 64 : A.k, in);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < S::VK; u++) {
+            const int j = first + (u >> 1) * 8 + 2 * t + (u & 1), p = __shfl_sync(FULL, ids, (j >> shift) - base);
+            const bool ok = c.visible(j) && p >= 0 && p < A.c.n_pages;
+            const char* src = ok ? vb + p * A.c.v_page * SZ + (static_cast<long>(j & (A.c.page - 1)) * ncv + g) * 16 : A.v;
+#pragma unroll
+            for (int x = 0; x < S::VCH; x++) {
+                const bool in = ok && x * 8 + g < ncv;
+                if (x * 8 < ncv) cp16(dst + (S::KT * S::KCH + u * S::VCH + x) * 512, in ? src + x * 128 : A.v, in);
+            }
+        }
+        return good;
     }
+};
 
-    // q of head g: lane t holds the elements that its K chunks hold
+// One tile of query heads against the cache: q's parts, and the running maximum (in base 2), sum and output. Lane
+// (g, t) holds head g; after the last step its sum is that of its own columns only, and its outputs are the elements
+// 8 EPC c + 2 EPC t + e (o[2 EPC c + e], e < 2 EPC) of the head.
+template <int TYPE, int D>
+struct Tile {
+    using S = Shape<TYPE, D>;
     uint32_t qp[S::PARTS][S::QP];
-    float qscale = A.scale2, off = 0.0f;
-    {
+    float o[D / 4];
+    float m, l, qscale, off;
+
+    // x: the head's q, lane t the elements that its K chunks hold
+    __device__ __forceinline__ void start(const PagedArgs& A, const Cursor<TYPE, D>& c) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        const int kvh = c.unit / A.chunks, head0 = kvh * A.G + (c.unit - kvh * A.chunks) * A.per_chunk;
+        const int heads = min(A.per_chunk, (kvh + 1) * A.G - head0);
+        const float* qr = A.q + static_cast<long>(c.row) * A.ldq + static_cast<long>(head0 + min(g, heads - 1)) * A.c.dk;
         float x[S::QW];
-        const float* qr = A.q + static_cast<long>(row) * A.ldq + static_cast<long>(head0 + min(g, heads - 1)) * A.c.dk;
 #pragma unroll
-        for (int c = 0; c < S::KCH; c++)
+        for (int k = 0; k < S::KCH; k++)
 #pragma unroll
             for (int e = 0; e < S::EPC; e += 4) {
-                const int d = (c * 4 + t) * S::EPC + e;
+                const int d = (k * 4 + t) * S::EPC + e;
                 float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (d < A.c.dk) f = A.vecq ? *reinterpret_cast<const float4*>(qr + d) : make_float4(qr[d], qr[d + 1], qr[d + 2], qr[d + 3]);
-                x[c * S::EPC + e] = f.x;
-                x[c * S::EPC + e + 1] = f.y;
-                x[c * S::EPC + e + 2] = f.z;
-                x[c * S::EPC + e + 3] = f.w;
+                x[k * S::EPC + e] = f.x;
+                x[k * S::EPC + e + 1] = f.y;
+                x[k * S::EPC + e + 2] = f.z;
+                x[k * S::EPC + e + 3] = f.w;
             }
+        qscale = A.scale2;
+        off = 0.0f;
         if constexpr (TYPE == KX_KV_F16) {
             // |q| < 2^14 after the scaling; parts keep 22 bits of what is above 2^-17 of the head's largest element
-            float m = 0.0f;
+            float top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < S::QW; i++) m = fmaxf(m, fabsf(x[i]));
-            m = fmaxf(m, __shfl_xor_sync(FULL, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(FULL, m, 2));
-            const int e = min(max(static_cast<int>(__float_as_uint(m) >> 23) - 127, -100), 126);  // floor(log2 m)
+            for (int k = 0; k < S::QW; k++) top = fmaxf(top, fabsf(x[k]));
+            top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+            const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 126);  // floor(log2 top)
             const float up = __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
             qscale *= __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
             off = 13.0f;
 #pragma unroll
-            for (int i = 0; i < S::QW; i++) x[i] *= up;
+            for (int k = 0; k < S::QW; k++) x[k] *= up;
         }
         if constexpr (TYPE == KX_KV_F32) {
 #pragma unroll
-            for (int i = 0; i < S::QW; i++) {
+            for (int k = 0; k < S::QW; k++) {
                 float lo;
-                qp[0][i] = tf32_of(x[i], &lo);
-                qp[1][i] = __float_as_uint(lo);
+                qp[0][k] = tf32_of(x[k], &lo);
+                qp[1][k] = __float_as_uint(lo);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < S::QP; i++) {
-                float a = x[2 * i], b = x[2 * i + 1];
+            for (int k = 0; k < S::QP; k++) {
+                float a = x[2 * k], b = x[2 * k + 1];
 #pragma unroll
-                for (int p = 0; p < S::PARTS; p++) qp[p][i] = pack2<TYPE>(a, b, &a, &b);
+                for (int p = 0; p < S::PARTS; p++) qp[p][k] = pack2<TYPE>(a, b, &a, &b);
             }
         }
+#pragma unroll
+        for (int k = 0; k < D / 4; k++) o[k] = 0.0f;
+        m = -INFINITY;
+        l = 0.0f;
     }
 
-    float o[D / 4];
-#pragma unroll
-    for (int i = 0; i < D / 4; i++) o[i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    int stage = 0;
-    for (int i = i0 + warp; i < i1; i += PG_WARPS) {
-        {
-            const int ahead = i + (PG_STAGES - 1) * PG_WARPS;
-            const int next = page_of(ahead + PG_WARPS);
-            issue(ahead, pid, stage == 0 ? PG_STAGES - 1 : stage - 1);
-            pid = next;
-        }
-        cp_wait<PG_STAGES - 1>();
-        const uint32_t src = ring + stage * S::STAGE;
-        stage = stage + 1 == PG_STAGES ? 0 : stage + 1;
-
+    // a step whose chunks lie at shared address src
+    __device__ __forceinline__ void step(const Cursor<TYPE, D>& c, uint32_t src, int nck, int ncv) {
+        const int t = threadIdx.x & 3;
         // scores: rows 0-7 and 8-15 of the tile are the products of q's parts
         float s[2 * S::KT];
 #pragma unroll
         for (int u = 0; u < S::KT; u++) {
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            float dd[2][4] = {};  // two chains of products
 #pragma unroll
-            for (int c = 0; c < S::KCH; c++) {
-                if (c * 4 >= nck) continue;
-                const uint4 kv = lds16(src + (u * S::KCH + c) * 512);
+            for (int k = 0; k < S::KCH; k++) {
+                if (k * 4 >= nck) continue;
+                float(&d)[4] = dd[k & 1];
+                const uint4 kv = lds16(src + (u * S::KCH + k) * 512);
+                const int x = k * 4;
                 if constexpr (TYPE == KX_KV_F32) {
                     const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int x = c * 4 + 2 * h;
+                    for (int h = 0; h < 4; h += 2) {
                         float l0, l1;
-                        const uint32_t h0 = tf32_of(__uint_as_float(w[2 * h]), &l0), h1 = tf32_of(__uint_as_float(w[2 * h + 1]), &l1);
-                        mma_tf32(d, qp[0][x], qp[1][x], qp[0][x + 1], qp[1][x + 1], h0, h1);
-                        mma_tf32(d, qp[0][x], 0, qp[0][x + 1], 0, __float_as_uint(l0), __float_as_uint(l1));
+                        const uint32_t h0 = tf32_of(__uint_as_float(w[h]), &l0), h1 = tf32_of(__uint_as_float(w[h + 1]), &l1);
+                        mma_tf32(d, qp[0][x + h], qp[1][x + h], qp[0][x + h + 1], qp[1][x + h + 1], h0, h1);
+                        mma_tf32(d, qp[0][x + h], 0, qp[0][x + h + 1], 0, __float_as_uint(l0), __float_as_uint(l1));
                     }
+                } else if constexpr (TYPE == KX_KV_F16) {
+                    mma_f16(d, qp[0][x], qp[1][x], qp[0][x + 1], qp[1][x + 1], kv.x, kv.y);
+                    mma_f16(d, qp[0][x + 2], qp[1][x + 2], qp[0][x + 3], qp[1][x + 3], kv.z, kv.w);
                 } else {
-                    const int x = c * 4;
-                    if constexpr (TYPE == KX_KV_F16) {
-                        mma_f16(d, qp[0][x], qp[1][x], qp[0][x + 1], qp[1][x + 1], kv.x, kv.y);
-                        mma_f16(d, qp[0][x + 2], qp[1][x + 2], qp[0][x + 3], qp[1][x + 3], kv.z, kv.w);
-                    } else {
-                        mma_bf16(d, qp[0][x], qp[1][x], qp[0][x + 1], qp[1][x + 1], kv.x, kv.y);
-                        mma_bf16(d, qp[0][x + 2], qp[1][x + 2], qp[0][x + 3], qp[1][x + 3], kv.z, kv.w);
-                        mma_bf16(d, qp[2][x], 0, qp[2][x + 1], 0, kv.x, kv.y);
-                        mma_bf16(d, qp[2][x + 2], 0, qp[2][x + 3], 0, kv.z, kv.w);
-                    }
+                    mma_bf16(d, qp[0][x], qp[1][x], qp[0][x + 1], qp[1][x + 1], kv.x, kv.y);
+                    mma_bf16(d, qp[0][x + 2], qp[1][x + 2], qp[0][x + 3], qp[1][x + 3], kv.z, kv.w);
+                    mma_bf16(d, qp[2][x], 0, qp[2][x + 1], 0, kv.x, kv.y);
+                    mma_bf16(d, qp[2][x + 2], 0, qp[2][x + 3], 0, kv.z, kv.w);
                 }
             }
-            const int j = first_key(i) + u * 8 + 2 * t;
-            s[2 * u] = visible(j) ? (d[0] + d[2]) * qscale : -INFINITY;
-            s[2 * u + 1] = visible(j + 1) ? (d[1] + d[3]) * qscale : -INFINITY;
+            s[2 * u] = ((dd[0][0] + dd[1][0]) + (dd[0][2] + dd[1][2])) * qscale;
+            s[2 * u + 1] = ((dd[0][1] + dd[1][1]) + (dd[0][3] + dd[1][3])) * qscale;
+        }
+        if (!c.whole()) {
+            const int j = c.first_key() + 2 * t;
+#pragma unroll
+            for (int e = 0; e < 2 * S::KT; e++)
+                if (!c.visible(j + (e >> 1) * 8 + (e & 1))) s[e] = -INFINITY;
         }
         float mx = s[0];
 #pragma unroll
@@ -360,43 +413,43 @@ __device__ void paged_piece(const PagedArgs& A, uint8_t* smem, float (&red)[PG_W
             p[e] = kx::ex2(s[e] - (safe - off));
             l += p[e];
         }
-
-        // p.v: column 2 t (2 t + 1) of n-tile (c, e) is element e of chunk 8 c + 2 t (+ 1)
+        // p.v: column 2 t (2 t + 1) of n-tile (k, e) is element e of chunk 8 k + 2 t (+ 1)
+        const uint32_t vsrc = src + S::KT * S::KCH * 512;
         if constexpr (TYPE == KX_KV_F32) {
             float q0, q1;
             const uint32_t h0 = tf32_of(p[0], &q0), h1 = tf32_of(p[1], &q1);
 #pragma unroll
-            for (int c = 0; c < S::VCH; c++) {
-                if (c * 8 >= ncv) continue;
-                const uint4 va = lds16(src + (S::KT * S::KCH + c) * 512), vbq = lds16(src + (S::KT * S::KCH + S::VCH + c) * 512);
-                const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vbq.x, vbq.y, vbq.z, vbq.w};
+            for (int k = 0; k < S::VCH; k++) {
+                if (k * 8 >= ncv) continue;
+                const uint4 va = lds16(vsrc + k * 512), vb = lds16(vsrc + (S::VCH + k) * 512);
+                const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     float d[4] = {0.f, 0.f, 0.f, 0.f}, l0, l1;
                     const uint32_t v0 = tf32_of(__uint_as_float(wa[e]), &l0), v1 = tf32_of(__uint_as_float(wb[e]), &l1);
                     mma_tf32(d, h0, 0, h1, 0, __float_as_uint(l0), __float_as_uint(l1));
                     mma_tf32(d, h0, __float_as_uint(q0), h1, __float_as_uint(q1), v0, v1);
-                    o[c * 8 + e] += d[0] + d[2];
-                    o[c * 8 + 4 + e] += d[1] + d[3];
+                    o[k * 8 + e] += d[0] + d[2];
+                    o[k * 8 + 4 + e] += d[1] + d[3];
                 }
             }
         } else {
             uint32_t pa[S::PARTS], pb[S::PARTS];
             {
-                float a = p[0], b = p[1], c = p[2], d = p[3];
+                float a = p[0], b = p[1], cc = p[2], d = p[3];
 #pragma unroll
                 for (int x = 0; x < S::PARTS; x++) {
                     pa[x] = pack2<TYPE>(a, b, &a, &b);
-                    pb[x] = pack2<TYPE>(c, d, &c, &d);
+                    pb[x] = pack2<TYPE>(cc, d, &cc, &d);
                 }
             }
 #pragma unroll
-            for (int c = 0; c < S::VCH; c++) {
-                if (c * 8 >= ncv) continue;
+            for (int k = 0; k < S::VCH; k++) {
+                if (k * 8 >= ncv) continue;
                 uint32_t w[4][4];
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
-                    const uint4 x = lds16(src + (S::KT * S::KCH + u * S::VCH + c) * 512);
+                    const uint4 x = lds16(vsrc + (u * S::VCH + k) * 512);
                     w[u][0] = x.x, w[u][1] = x.y, w[u][2] = x.z, w[u][3] = x.w;
                 }
 #pragma unroll
@@ -410,33 +463,91 @@ __device__ void paged_piece(const PagedArgs& A, uint8_t* smem, float (&red)[PG_W
                         mma_bf16(d, pa[2], 0, pb[2], 0, b0, b1);
                         mma_bf16(d, pa[0], pa[1], pb[0], pb[1], b0, b1);
                     }
-                    o[c * 16 + e] += d[0] + d[2];
-                    o[c * 16 + 8 + e] += d[1] + d[3];
+                    o[k * 16 + e] += d[0] + d[2];
+                    o[k * 16 + 8 + e] += d[1] + d[3];
                 }
             }
         }
     }
-    cp_wait<0>();
 
-    // the warps' partial results meet in shared memory (each in the place of its own ring)
-    bad = __any_sync(FULL, bad);
-    l += __shfl_xor_sync(FULL, l, 1);
-    l += __shfl_xor_sync(FULL, l, 2);
-    __syncwarp();
-    if (t == 0) {
-        red[warp][g][0] = m;
-        red[warp][g][1] = bad ? NAN : l;
+    __device__ __forceinline__ void finish(bool bad) {
+        l += __shfl_xor_sync(FULL, l, 1);
+        l += __shfl_xor_sync(FULL, l, 2);
+        if (bad) l = NAN;
     }
+    // outputs e .. e + 3 of chunk group k: element d of the head
+    __device__ __forceinline__ static int element(int k, int e) { return k * 8 * S::EPC + (threadIdx.x & 3) * 2 * S::EPC + e; }
+    __device__ __forceinline__ float4 four(int k, int e, float f) const {
+        const float* x = o + k * 2 * S::EPC + e;
+        return make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+    }
+};
+
+constexpr size_t PG_PART = (PG_HEADS * PG_DMAX + 2 * PG_HEADS) * sizeof(float);
+__device__ __host__ inline size_t part_offset(int warp, int which) {
+    return PG_MAX_WARPS * sizeof(PagedDesc) + (static_cast<size_t>(warp) * 2 + which) * PG_PART;
+}
+
+__device__ __forceinline__ int tile_heads(const PagedArgs& A, int unit, int* head0) {
+    const int kvh = unit / A.chunks;
+    *head0 = kvh * A.G + (unit - kvh * A.chunks) * A.per_chunk;
+    return min(A.per_chunk, (kvh + 1) * A.G - *head0);
+}
+
+// Short sequences: one CTA per unit, its warps take every fourth step and meet in shared memory.
+template <int TYPE, int D>
+__global__ void __launch_bounds__(PG_THREADS, 2) k_paged_unit(const PagedArgs A) {
+    using S = Shape<TYPE, D>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float red[PG_WARPS][PG_HEADS][2];
+    const int units = A.c.heads * A.chunks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int nck = A.c.dk / S::EPC, ncv = A.c.dv / S::EPC, shift = 31 - __clz(A.c.page);
+    kx::griddep_wait();
+    kx::griddep_launch_dependents();
+    Cursor<TYPE, D> c;
+    c.row = blockIdx.x / units;
+    c.unit = blockIdx.x - c.row * units;
+    c.sp = span_of<S::KS>(A, c.row, &c.slot);
+    if (c.sp.steps == 0) return;
+    const uint32_t ring = kx::smem_u32(smem) + warp * (PG_STAGES * S::STAGE) + lane * 16;
+    Feed<TYPE, D> feed;
+    feed.unit(A, c);
+    bool bad = c.sp.bad;
+    Cursor<TYPE, D> ahead = c;
+    ahead.i = warp;
+    const auto issue = [&](int stage) {
+        if (ahead.i < c.sp.steps && !feed.issue(A, ahead, ring + stage * S::STAGE, nck, ncv, shift)) bad = true;
+        ahead.i += PG_WARPS;
+        cp_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < PG_STAGES - 1; s++) issue(s);
+    Tile<TYPE, D> tile;
+    tile.start(A, c);
+    int stage = 0;
+    for (c.i = warp; c.i < c.sp.steps; c.i += PG_WARPS) {
+        issue(stage == 0 ? PG_STAGES - 1 : stage - 1);
+        cp_wait<PG_STAGES - 1>();
+        tile.step(c, ring + stage * S::STAGE, nck, ncv);
+        stage = stage + 1 == PG_STAGES ? 0 : stage + 1;
+    }
+    cp_wait<0>();
+    bad = __any_sync(FULL, bad);
     if (bad && lane == 0) kx::kv_report(A.status, KX_STATUS_BAD_REQUEST);
-    float* mine = reinterpret_cast<float*>(smem + warp * (PG_STAGES * S::STAGE));
-    // lane (g, t): 2 EPC contiguous elements of head g per V chunk group
+    tile.finish(bad);
+    if (t == 0) {
+        red[warp][g][0] = tile.m;
+        red[warp][g][1] = tile.l;
+    }
+    __syncwarp();
+    float* mine = reinterpret_cast<float*>(smem + warp * (PG_STAGES * S::STAGE));  // the warp's ring, no longer in use
 #pragma unroll
-    for (int c = 0; c < S::VCH; c++)
+    for (int k = 0; k < S::VCH; k++)
 #pragma unroll
-        for (int e = 0; e < 2 * S::EPC; e += 4)
-            *reinterpret_cast<float4*>(mine + g * D + c * 8 * S::EPC + t * 2 * S::EPC + e) =
-                make_float4(o[c * 2 * S::EPC + e], o[c * 2 * S::EPC + e + 1], o[c * 2 * S::EPC + e + 2], o[c * 2 * S::EPC + e + 3]);
+        for (int e = 0; e < 2 * S::EPC; e += 4) *reinterpret_cast<float4*>(mine + g * D + tile.element(k, e)) = tile.four(k, e, 1.0f);
     __syncthreads();
+    int head0;
+    const int heads = tile_heads(A, c.unit, &head0);
     for (int x = tid; x < heads * D; x += PG_THREADS) {
         const int h = x / D, d = x - h * D;
         float mm = red[0][h][0];
@@ -450,158 +561,247 @@ __device__ void paged_piece(const PagedArgs& A, uint8_t* smem, float (&red)[PG_W
             den += f * red[w][h][1];
             num += f * reinterpret_cast<const float*>(smem + w * (PG_STAGES * S::STAGE))[x];
         }
-        if (part) {
-            part[x] = num;
-            if (d == 0) {
-                part[PG_HEADS * PG_DMAX + 2 * h] = mm;
-                part[PG_HEADS * PG_DMAX + 2 * h + 1] = den;
-            }
-        } else if (d < A.c.dv) {
-            A.ctx[static_cast<long>(row) * A.ldc + static_cast<long>(head0 + h) * A.c.dv + d] = den == 0.0f ? 0.0f : num / den;
-        }
+        if (d < A.c.dv) A.ctx[static_cast<long>(c.row) * A.ldc + static_cast<long>(head0 + h) * A.c.dv + d] = den == 0.0f ? 0.0f : num / den;
     }
-    __syncthreads();  // the rings and `red` are free for the next piece
 }
 
-constexpr size_t PG_PART = (PG_HEADS * PG_DMAX + 2 * PG_HEADS) * sizeof(float);
-__device__ __host__ inline size_t part_offset(int cta, int which) {
-    return PG_MAX_CTAS * sizeof(PagedDesc) + (static_cast<size_t>(cta) * 2 + which) * PG_PART;
-}
-
-__device__ __forceinline__ long long warp_sum(long long v) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(FULL, v, d);
-    return v;
-}
-
-// SPLIT: CTA j takes the steps [j per, (j + 1) per) of the line; otherwise CTA j is one unit
-template <int TYPE, int D, bool SPLIT>
-__global__ void __launch_bounds__(PG_THREADS, 2) k_paged(const PagedArgs A) {
+// Warp w of the launch takes the steps [w per, (w + 1) per) of the line, whatever units they belong to; the loads run
+// ahead of the products across the units' ends.
+template <int TYPE, int D>
+__global__ void __launch_bounds__(PG_THREADS, 2) k_paged_line(const PagedArgs A) {
     using S = Shape<TYPE, D>;
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float red[PG_WARPS][PG_HEADS][2];
+    __shared__ long long upto[PG_THREADS];
     __shared__ long long sums[PG_WARPS];
-    __shared__ long long found_first;
-    __shared__ int found_row;
-    const int units = A.c.heads * A.chunks, tid = threadIdx.x, lane = tid & 31;
+    const int units = A.c.heads * A.chunks, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int nck = A.c.dk / S::EPC, ncv = A.c.dv / S::EPC, shift = 31 - __clz(A.c.page);
     kx::griddep_wait();
     kx::griddep_launch_dependents();
-    int slot;
-    if constexpr (!SPLIT) {
-        const int row = blockIdx.x / units;
-        const Span sp = span_of<S::KS>(A, row, &slot);
-        if (slot < 0) return;
-        paged_piece<TYPE, D>(A, smem, red, row, slot < A.c.n_seqs ? slot : 0, sp, blockIdx.x - row * units, 0, sp.steps, nullptr);
-        return;
-    }
-    // the line's length, then the row that this CTA's range begins in
-    long long mine = 0;
-    for (int r = tid; r < A.n; r += PG_THREADS) mine += span_of<S::KS>(A, r, &slot).steps;
-    mine = warp_sum(mine);
-    if (lane == 0) sums[tid >> 5] = mine;
-    if (tid == 0) found_row = -1;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < PG_WARPS; w++) total += sums[w];
-    total *= units;
-    const long long per = max((total + A.grid - 1) / A.grid, static_cast<long long>(PG_MIN_STEPS));
-    const long long lo = blockIdx.x * per, hi = min(lo + per, total);
-    PagedDesc* desc = reinterpret_cast<PagedDesc*>(A.ws) + blockIdx.x;
-    if (lo >= total) {
-        if (tid == 0) desc->row = -1;
-        return;
-    }
-    long long before = 0;
-    for (int r0 = 0; r0 < A.n; r0 += PG_THREADS) {
+
+    // rows r0 .. r0 + PG_THREADS - 1: upto[x] = steps per unit of the rows r0 .. r0 + x; returns the last of them
+    const auto scan_rows = [&](int r0) {
+        int slot;
         const int r = r0 + tid;
-        const long long st = r < A.n ? static_cast<long long>(span_of<S::KS>(A, r, &slot).steps) * units : 0;
-        long long incl = st;
+        long long v = r < A.n ? span_of<S::KS>(A, r, &slot).steps : 0;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const long long u = __shfl_up_sync(FULL, incl, d);
-            if (lane >= d) incl += u;
+            const long long u = __shfl_up_sync(FULL, v, d);
+            if (lane >= d) v += u;
         }
         __syncthreads();
-        if (lane == 31) sums[tid >> 5] = incl;
+        if (lane == 31) sums[warp] = v;
         __syncthreads();
         long long all = 0;
 #pragma unroll
         for (int w = 0; w < PG_WARPS; w++) {
-            if (w < (tid >> 5)) incl += sums[w];
+            if (w < warp) v += sums[w];
             all += sums[w];
         }
-        incl += before;
-        if (lo < incl && lo >= incl - st) {
-            found_row = r;
-            found_first = incl - st;
+        upto[tid] = v;
+        __syncthreads();
+        return all;
+    };
+    long long total = 0;
+    for (int r0 = 0; r0 < A.n; r0 += PG_THREADS) total += scan_rows(r0);
+    total *= units;
+    const int me = blockIdx.x * PG_WARPS + warp, warps = gridDim.x * PG_WARPS;
+    const long long per = max((total + warps - 1) / warps, static_cast<long long>(PG_MIN_STEPS));
+    const long long lo = me * per, hi = min(lo + per, total);
+    Cursor<TYPE, D> c;
+    c.row = -1;
+    long long first = 0;  // the row's first step on the line
+    long long before = 0;
+    for (int r0 = 0; r0 < A.n; r0 += PG_THREADS) {  // the row that lo lies in
+        const long long all = A.n > PG_THREADS ? scan_rows(r0) : total / units;
+        if (c.row < 0 && lo < total && lo < (before + all) * units) {
+#pragma unroll
+            for (int x = 0; x < PG_THREADS; x += 32) {
+                const unsigned hit = __ballot_sync(FULL, lo < (before + upto[x + lane]) * units);
+                if (hit) {
+                    const int at = x + __ffs(hit) - 1;
+                    c.row = r0 + at;
+                    first = (before + (at ? upto[at - 1] : 0)) * units;
+                    break;
+                }
+            }
         }
         before += all;
-        if (lo < before) break;
     }
-    __syncthreads();
-    int row = found_row;
-    long long first = found_first;  // the row's first step on the line
-    for (long long at = lo; at < hi; row++) {
-        const Span sp = span_of<S::KS>(A, row, &slot);
-        if (slot < 0) continue;
-        int unit = static_cast<int>((at - first) / sp.steps);
-        for (; unit < units && at < hi; unit++) {
-            const long long u0 = first + static_cast<long long>(unit) * sp.steps, u1 = u0 + sp.steps;
-            if (at == lo && tid == 0) *desc = PagedDesc{u0, per, row, unit, sp.steps, 0};
-            const long long end = min(u1, hi);
-            float* part = nullptr;  // a unit in several ranges: its first part in place 1, the others in place 0
-            if (at != u0 || end != u1) part = reinterpret_cast<float*>(A.ws + part_offset(blockIdx.x, at == u0));
-            paged_piece<TYPE, D>(A, smem, red, row, slot < A.c.n_seqs ? slot : 0, sp, unit, static_cast<int>(at - u0),
-                                 static_cast<int>(end - u0), part);
-            at = end;
+    PagedDesc* desc = reinterpret_cast<PagedDesc*>(A.ws) + me;
+    if (c.row < 0) {
+        if (lane == 0) desc->row = -1;
+        return;
+    }
+    c.sp = span_of<S::KS>(A, c.row, &c.slot);
+    c.unit = static_cast<int>((lo - first) / c.sp.steps);
+    c.i = static_cast<int>(lo - first - static_cast<long long>(c.unit) * c.sp.steps);
+    if (lane == 0) *desc = PagedDesc{lo - c.i, per, c.row, c.unit, c.sp.steps, 0};
+
+    const uint32_t ring = kx::smem_u32(smem) + warp * (PG_STAGES * S::STAGE) + lane * 16;
+    const int count = static_cast<int>(hi - lo);
+    Cursor<TYPE, D> ahead = c;
+    Feed<TYPE, D> feed;
+    feed.unit(A, ahead);
+    int sent = 0;
+    unsigned missing = 0;  // per stage: a page was not there
+    const auto issue = [&](int stage) {
+        if (sent < count) {
+            const bool good = feed.issue(A, ahead, ring + stage * S::STAGE, nck, ncv, shift);
+            missing = (missing & ~(1u << stage)) | (good ? 0u : 1u << stage);
+            if (++sent < count && !ahead.next(A, units)) feed.unit(A, ahead);
         }
-        first += static_cast<long long>(sp.steps) * units;
+        cp_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < PG_STAGES - 1; s++) issue(s);
+    Tile<TYPE, D> tile;
+    int stage = 0;
+    for (int done = 0; done < count;) {
+        const int i0 = c.i, steps = min(c.sp.steps - c.i, count - done);
+        bool bad = c.sp.bad;
+        tile.start(A, c);
+        for (int x = 0; x < steps; x++) {
+            issue(stage == 0 ? PG_STAGES - 1 : stage - 1);
+            cp_wait<PG_STAGES - 1>();
+            bad = bad || (missing >> stage & 1);
+            c.i = i0 + x;
+            tile.step(c, ring + stage * S::STAGE, nck, ncv);
+            stage = stage + 1 == PG_STAGES ? 0 : stage + 1;
+        }
+        bad = __any_sync(FULL, bad);
+        if (bad && lane == 0) kx::kv_report(A.status, KX_STATUS_BAD_REQUEST);
+        tile.finish(bad);
+        int head0;
+        const int heads = tile_heads(A, c.unit, &head0);
+        if (g < heads) {
+            if (steps == c.sp.steps) {
+                const float inv = tile.l == 0.0f ? 0.0f : 1.0f / tile.l;
+                float* out = A.ctx + static_cast<long>(c.row) * A.ldc + static_cast<long>(head0 + g) * A.c.dv;
+#pragma unroll
+                for (int k = 0; k < S::VCH; k++)
+#pragma unroll
+                    for (int e = 0; e < 2 * S::EPC; e += 4) {
+                        const int d = tile.element(k, e);
+                        if (d >= A.c.dv) continue;
+                        const float4 f = tile.four(k, e, inv);
+                        if (A.vecc) {
+                            *reinterpret_cast<float4*>(out + d) = f;
+                        } else {
+                            out[d] = f.x, out[d + 1] = f.y, out[d + 2] = f.z, out[d + 3] = f.w;
+                        }
+                    }
+            } else {  // a unit in several ranges: its first part in place 1, the others in place 0
+                float* part = reinterpret_cast<float*>(A.ws + part_offset(me, i0 == 0));
+#pragma unroll
+                for (int k = 0; k < S::VCH; k++)
+#pragma unroll
+                    for (int e = 0; e < 2 * S::EPC; e += 4)
+                        *reinterpret_cast<float4*>(part + g * D + tile.element(k, e)) = tile.four(k, e, 1.0f);
+                if (t == 0) *reinterpret_cast<float2*>(part + PG_HEADS * PG_DMAX + 2 * g) = make_float2(tile.m, tile.l);
+            }
+        }
+        done += steps;
+        if (done < count) c.next(A, units);
     }
 }
 
-// CTA (j, h): if the range of CTA j + 1 begins inside a unit whose first step lies in the range of CTA j, joins that
-// unit's parts for head h, in their order: each warp every 4th part, then the warps.
-__global__ void __launch_bounds__(128) k_paged_join(const PagedArgs A) {
-    __shared__ float acc[4][PG_DMAX];
-    __shared__ float ml[4][2];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y;
-    kx::griddep_wait();
-    const PagedDesc ds = reinterpret_cast<const PagedDesc*>(A.ws)[blockIdx.x + 1];
-    if (ds.row < 0) return;
-    const long long j0 = ds.first / ds.per, j1 = (ds.first + ds.steps - 1) / ds.per;
-    if (j0 != blockIdx.x || ds.first == (blockIdx.x + 1) * ds.per) return;
-    const int kvh = ds.unit / A.chunks, head0 = kvh * A.G + (ds.unit - kvh * A.chunks) * A.per_chunk;
-    if (h >= min(A.per_chunk, (kvh + 1) * A.G - head0)) return;
-    const int D = A.c.dk <= 64 && A.c.dv <= 64 ? 64 : 128;
-    const int d = lane * 4;
-    const auto part = [&](long long j) { return reinterpret_cast<const float*>(A.ws + part_offset(static_cast<int>(j), j == j0)); };
+// A unit's parts j .. j1 (warps of the line) for head h, every `stride`-th from j + begin on: sum and output (4 elements
+// per lane, in the parts' order) relative to the largest maximum of all parts.
+__device__ __forceinline__ void join_parts(const PagedArgs& A, int j, int j1, int h, int begin, int stride, int D, float4* num, float* den) {
+    const int lane = threadIdx.x & 31, d = lane * 4;
+    const auto part = [&](int i) { return reinterpret_cast<const float*>(A.ws + part_offset(i, i == j)); };
     float m = -INFINITY;
-    for (long long j = j0 + lane; j <= j1; j += 32) m = fmaxf(m, __ldcg(part(j) + PG_HEADS * PG_DMAX + 2 * h));
+    for (int i = j + lane; i <= j1; i += 32) m = fmaxf(m, __ldcg(part(i) + PG_HEADS * PG_DMAX + 2 * h));
 #pragma unroll
-    for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, x));
+    for (int z = 16; z; z >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, z));
     const float ms = m == -INFINITY ? 0.0f : m;
-    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-    float den = 0.0f;
+    *num = make_float4(0.f, 0.f, 0.f, 0.f);
+    *den = 0.0f;
 #pragma unroll 4
-    for (long long j = j0 + warp; j <= j1; j += 4) {
-        const float* p = part(j);
+    for (int i = j + begin; i <= j1; i += stride) {
+        const float* p = part(i);
         const float2 st = __ldcg(reinterpret_cast<const float2*>(p + PG_HEADS * PG_DMAX + 2 * h));
         const float f = kx::ex2(st.x - ms);
         const float4 v = d < D ? __ldcg(reinterpret_cast<const float4*>(p + h * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        den += f * st.y;
-        num.x += f * v.x;
-        num.y += f * v.y;
-        num.z += f * v.z;
-        num.w += f * v.w;
+        *den += f * st.y;
+        num->x += f * v.x;
+        num->y += f * v.y;
+        num->z += f * v.z;
+        num->w += f * v.w;
     }
-    *reinterpret_cast<float4*>(&acc[warp][d]) = num;
-    if (lane == 0) ml[warp][0] = den;
-    __syncthreads();
-    const int x = threadIdx.x;
-    if (x < A.c.dv) {
-        const float n = acc[0][x] + acc[1][x] + acc[2][x] + acc[3][x], l = ml[0][0] + ml[1][0] + ml[2][0] + ml[3][0];
-        A.ctx[static_cast<long>(ds.row) * A.ldc + static_cast<long>(head0 + h) * A.c.dv + x] = l == 0.0f ? 0.0f : n / l;
+}
+
+// Tasks (warp j of the line, head h): if the range of warp j + 1 begins inside a unit whose first step lies in the range
+// of warp j, that unit's parts are joined for head h: by one warp where they are few, else by the CTA's eight, each
+// every eighth part, then the warps' sums in order.
+__global__ void __launch_bounds__(256) k_paged_join(const PagedArgs A, int warps) {
+    __shared__ float acc[8][PG_DMAX];
+    __shared__ float sum[8];
+    __shared__ int todo[2][32], n_todo[2];  // few parts, many parts
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    kx::griddep_wait();
+    const PagedDesc* desc = reinterpret_cast<const PagedDesc*>(A.ws);
+    const int tasks = (warps - 1) * A.per_chunk, D = A.c.dk <= 64 && A.c.dv <= 64 ? 64 : 128;
+    for (int t0 = blockIdx.x; t0 < tasks; t0 += gridDim.x * 32) {
+        if (warp == 0) {
+            const int task = t0 + lane * gridDim.x;
+            bool hit = false, many = false;
+            if (task < tasks) {
+                const int j = task / A.per_chunk, h = task - j * A.per_chunk;
+                const long long first = __ldcg(&desc[j + 1].first), per = __ldcg(&desc[j + 1].per);
+                const int row = __ldcg(&desc[j + 1].row), unit = __ldcg(&desc[j + 1].unit), steps = __ldcg(&desc[j + 1].steps);
+                if (row >= 0) {
+                    int head0;
+                    hit = first >= j * per && first < (j + 1) * per && h < tile_heads(A, unit, &head0);
+                    many = first + steps > (j + 16) * per;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const unsigned hits = __ballot_sync(FULL, hit && many == (x == 1));
+                if (hit && many == (x == 1)) todo[x][__popc(hits & ((1u << lane) - 1))] = task;
+                if (lane == 0) n_todo[x] = __popc(hits);
+            }
+        }
+        __syncthreads();
+        const auto output = [&](const PagedDesc& ds, int h) {
+            int head0;
+            tile_heads(A, ds.unit, &head0);
+            return A.ctx + static_cast<long>(ds.row) * A.ldc + static_cast<long>(head0 + h) * A.c.dv;
+        };
+        for (int x = warp; x < n_todo[0]; x += 8) {
+            const int j = todo[0][x] / A.per_chunk, h = todo[0][x] - j * A.per_chunk;
+            const PagedDesc ds = desc[j + 1];
+            float4 num;
+            float den;
+            join_parts(A, j, static_cast<int>((ds.first + ds.steps - 1) / ds.per), h, 0, 1, D, &num, &den);
+            const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+            if (lane * 4 < A.c.dv) {
+                float* out = output(ds, h) + lane * 4;
+                out[0] = num.x * inv, out[1] = num.y * inv, out[2] = num.z * inv, out[3] = num.w * inv;
+            }
+        }
+        for (int x = 0; x < n_todo[1]; x++) {
+            const int j = todo[1][x] / A.per_chunk, h = todo[1][x] - j * A.per_chunk;
+            const PagedDesc ds = desc[j + 1];
+            float4 num;
+            float den;
+            join_parts(A, j, static_cast<int>((ds.first + ds.steps - 1) / ds.per), h, warp, 8, D, &num, &den);
+            *reinterpret_cast<float4*>(&acc[warp][lane * 4]) = num;
+            if (lane == 0) sum[warp] = den;
+            __syncthreads();
+            if (tid < A.c.dv) {
+                float n = 0.0f, l = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 8; w++) {
+                    n += acc[w][tid];
+                    l += sum[w];
+                }
+                output(ds, h)[tid] = l == 0.0f ? 0.0f : n / l;
+            }
+            __syncthreads();
+        }
+        __syncthreads();  // todo is free for the next round
     }
 }
 
@@ -613,14 +813,14 @@ int launch(const PagedArgs& A, bool split, unsigned grid, cudaStream_t st) {
     if (cudaGetDevice(&dev) != cudaSuccess) return -1;
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(__atomic_load_n(&devs_set, __ATOMIC_ACQUIRE) & bit)) {
-        if (cudaFuncSetAttribute(k_paged<TYPE, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-            cudaFuncSetAttribute(k_paged<TYPE, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        if (cudaFuncSetAttribute(k_paged_line<TYPE, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            cudaFuncSetAttribute(k_paged_unit<TYPE, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
             return -1;
         __atomic_fetch_or(&devs_set, bit, __ATOMIC_RELEASE);
     }
-    if (!split) return kx::launch_pdl(k_paged<TYPE, D, false>, dim3(grid), dim3(PG_THREADS), smem, st, A);
-    if (kx::launch_pdl(k_paged<TYPE, D, true>, dim3(grid), dim3(PG_THREADS), smem, st, A) != 0) return -1;
-    return kx::launch_pdl(k_paged_join, dim3(grid - 1, A.per_chunk), dim3(128), 0, st, A);
+    if (!split) return kx::launch_pdl(k_paged_unit<TYPE, D>, dim3(grid), dim3(PG_THREADS), smem, st, A);
+    if (kx::launch_pdl(k_paged_line<TYPE, D>, dim3(grid), dim3(PG_THREADS), smem, st, A) != 0) return -1;
+    return kx::launch_pdl(k_paged_join, dim3(grid), dim3(256), 0, st, A, static_cast<int>(grid * PG_WARPS));
 }
 
 template <int TYPE>
@@ -634,7 +834,7 @@ extern "C" {
 
 size_t kx_attention_paged_ws(const kx_kv* c, int H, int n) {
     if (!kx::kv_ok(c) || c->dk > PG_DMAX || c->dv > PG_DMAX || H < 1 || H % c->heads || n < 0) return 0;
-    return part_offset(PG_MAX_CTAS, 0);
+    return part_offset(PG_MAX_WARPS, 0);
 }
 
 int kx_attention_paged(const kx_kv* c, int layer, const float* q, int ldq, int H, const int32_t* seqs, int n, int window, int sinks,
@@ -666,19 +866,19 @@ int kx_attention_paged(const kx_kv* c, int layer, const float* q, int ldq, int H
     A.window = window;
     A.sinks = sinks;
     A.scale2 = (scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(c->dk)) : scale) * 1.4426950408889634f;
+    A.vecc = (ldc & 3) == 0 && (reinterpret_cast<uintptr_t>(ctx) & 15) == 0;
     A.vecq = (ldq & 3) == 0 && (c->dk & 3) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
     int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
         return -1;
     const long units = static_cast<long>(n) * c->heads * A.chunks;
     if (units > INT32_MAX) return -1;
-    // the most steps a head can have: where a range's least length covers them, a CTA per head needs no join
+    // the most steps a unit can have: few enough for one CTA, which then needs no join
     const int ks = c->type == KX_KV_F32 ? 8 : 16;
     long keys = static_cast<long>(c->max_pages) * c->page;
     if (window > 0) keys = std::min(keys, static_cast<long>(window) + sinks + 2 * ks);
-    const bool split = (keys + ks - 1) / ks > PG_MIN_STEPS;
-    A.grid = std::min(2 * sms, PG_MAX_CTAS);
-    const unsigned grid = split ? A.grid : static_cast<unsigned>(units);
+    const bool split = (keys + ks - 1) / ks > PG_UNIT_STEPS;
+    const unsigned grid = split ? std::min(2 * sms, PG_MAX_WARPS / PG_WARPS) : static_cast<unsigned>(units);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (c->type == KX_KV_F32) return launch_d<KX_KV_F32>(A, split, grid, st);
     if (c->type == KX_KV_F16) return launch_d<KX_KV_F16>(A, split, grid, st);
