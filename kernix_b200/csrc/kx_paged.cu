@@ -111,24 +111,18 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-    uint4 r;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(a) : "memory");
-    return r;
-}
-
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]));
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]));
 }
 __device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]));
 }
@@ -166,14 +160,16 @@ struct Shape {
     static constexpr int KS = 8 * KT;                       // keys per step
     static constexpr int KCH = D / EPC / 4;                 // K chunks per lane and tile: chunk 4 c + t of key g
     static constexpr int VK = 2 * KT;                       // V keys per lane: 2 t, 2 t + 1 of each tile
-    static constexpr int VCH = D / EPC / 8;                 // V chunks per lane and key: chunk 8 c + g
+    static constexpr int VCH = (D / EPC + 7) / 8;           // V chunks per lane and key: chunk 8 c + g
+    static constexpr int NO = VCH * 2 * EPC;                // output elements per lane
+    static constexpr int DV = VCH * 8 * EPC;                // a head's outputs, the padding included
     static constexpr int CH = KT * KCH + VK * VCH;
     static constexpr int STAGE = CH * 32 * 16;              // bytes per warp and stage
     static constexpr int QW = D / 4;                        // q elements per lane
     static constexpr int PARTS = TYPE == KX_KV_BF16 ? 3 : 2;
     static constexpr int QP = TYPE == KX_KV_F32 ? QW : QW / 2;  // 32-bit words per part
     static constexpr int SMEM = PG_WARPS * PG_STAGES * STAGE;
-    static_assert(PG_STAGES * STAGE >= PG_HEADS * D * 4, "a warp's ring holds its partial output");
+    static_assert(PG_STAGES * STAGE >= PG_HEADS * DV * 4, "a warp's ring holds its partial output");
 };
 
 // where a warp is on the line: step i of unit `unit` (key-value head x tile of heads) of row `row`
@@ -239,7 +235,6 @@ struct Feed {
                 const char* vs = vb + p * A.c.v_page * SZ + static_cast<long>((slot + 2 * t) * ncv + g) * 16;
 #pragma unroll
                 for (int x = 0; x < S::KCH; x++) {
-                    if (x * 4 >= nck) continue;
                     const bool in = x * 4 + t < nck;
                     const char* src = in ? ks + x * 64 : A.k;
 #pragma unroll
@@ -247,7 +242,6 @@ struct Feed {
                 }
 #pragma unroll
                 for (int x = 0; x < S::VCH; x++) {
-                    if (x * 8 >= ncv) continue;
                     const bool in = x * 8 + g < ncv;
                     const char* src = in ? vs + x * 128 : A.v;
 #pragma unroll
@@ -267,7 +261,7 @@ struct Feed {
 #pragma unroll
             for (int x = 0; x < S::KCH; x++) {
                 const bool in = ok && x * 4 + t < nck;
-                if (x * 4 < nck) cp16(dst + (u * S::KCH + x) * 512, in ? src + x * 64 : A.k, in);
+                cp16(dst + (u * S::KCH + x) * 512, in ? src + x * 64 : A.k, in);
             }
         }
 #pragma unroll
@@ -278,7 +272,7 @@ struct Feed {
 #pragma unroll
             for (int x = 0; x < S::VCH; x++) {
                 const bool in = ok && x * 8 + g < ncv;
-                if (x * 8 < ncv) cp16(dst + (S::KT * S::KCH + u * S::VCH + x) * 512, in ? src + x * 128 : A.v, in);
+                cp16(dst + (S::KT * S::KCH + u * S::VCH + x) * 512, in ? src + x * 128 : A.v, in);
             }
         }
         return good;
@@ -292,7 +286,7 @@ template <int TYPE, int D>
 struct Tile {
     using S = Shape<TYPE, D>;
     uint32_t qp[S::PARTS][S::QP];
-    float o[D / 4];
+    float o[S::NO];
     float m, l, qscale, off;
 
     // x: the head's q, lane t the elements that its K chunks hold
@@ -346,13 +340,13 @@ struct Tile {
             }
         }
 #pragma unroll
-        for (int k = 0; k < D / 4; k++) o[k] = 0.0f;
+        for (int k = 0; k < S::NO; k++) o[k] = 0.0f;
         m = -INFINITY;
         l = 0.0f;
     }
 
-    // a step whose chunks lie at shared address src
-    __device__ __forceinline__ void step(const Cursor<TYPE, D>& c, uint32_t src, int nck, int ncv) {
+    // a step whose chunks lie at src in shared memory
+    __device__ __forceinline__ void step(const Cursor<TYPE, D>& c, const uint8_t* src) {
         const int t = threadIdx.x & 3;
         // scores: rows 0-7 and 8-15 of the tile are the products of q's parts
         float s[2 * S::KT];
@@ -361,9 +355,8 @@ struct Tile {
             float dd[2][4] = {};  // two chains of products
 #pragma unroll
             for (int k = 0; k < S::KCH; k++) {
-                if (k * 4 >= nck) continue;
                 float(&d)[4] = dd[k & 1];
-                const uint4 kv = lds16(src + (u * S::KCH + k) * 512);
+                const uint4 kv = *reinterpret_cast<const uint4*>(src + (u * S::KCH + k) * 512);
                 const int x = k * 4;
                 if constexpr (TYPE == KX_KV_F32) {
                     const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
@@ -404,7 +397,7 @@ struct Tile {
             const float alpha = kx::ex2(m - safe);
             l *= alpha;
 #pragma unroll
-            for (int e = 0; e < D / 4; e++) o[e] *= alpha;
+            for (int e = 0; e < S::NO; e++) o[e] *= alpha;
         }
         m = mn;
         float p[2 * S::KT];
@@ -414,14 +407,13 @@ struct Tile {
             l += p[e];
         }
         // p.v: column 2 t (2 t + 1) of n-tile (k, e) is element e of chunk 8 k + 2 t (+ 1)
-        const uint32_t vsrc = src + S::KT * S::KCH * 512;
+        const uint8_t* vsrc = src + S::KT * S::KCH * 512;
         if constexpr (TYPE == KX_KV_F32) {
             float q0, q1;
             const uint32_t h0 = tf32_of(p[0], &q0), h1 = tf32_of(p[1], &q1);
 #pragma unroll
             for (int k = 0; k < S::VCH; k++) {
-                if (k * 8 >= ncv) continue;
-                const uint4 va = lds16(vsrc + k * 512), vb = lds16(vsrc + (S::VCH + k) * 512);
+                const uint4 va = *reinterpret_cast<const uint4*>(vsrc + k * 512), vb = *reinterpret_cast<const uint4*>(vsrc + (S::VCH + k) * 512);
                 const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -445,11 +437,10 @@ struct Tile {
             }
 #pragma unroll
             for (int k = 0; k < S::VCH; k++) {
-                if (k * 8 >= ncv) continue;
                 uint32_t w[4][4];
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
-                    const uint4 x = lds16(vsrc + (u * S::VCH + k) * 512);
+                    const uint4 x = *reinterpret_cast<const uint4*>(vsrc + (u * S::VCH + k) * 512);
                     w[u][0] = x.x, w[u][1] = x.y, w[u][2] = x.z, w[u][3] = x.w;
                 }
 #pragma unroll
@@ -509,7 +500,8 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_unit(const PagedArgs A)
     c.unit = blockIdx.x - c.row * units;
     c.sp = span_of<S::KS>(A, c.row, &c.slot);
     if (c.sp.steps == 0) return;
-    const uint32_t ring = kx::smem_u32(smem) + warp * (PG_STAGES * S::STAGE) + lane * 16;
+    const uint8_t* const chunks = smem + warp * (PG_STAGES * S::STAGE) + lane * 16;
+    const uint32_t ring = kx::smem_u32(chunks);
     Feed<TYPE, D> feed;
     feed.unit(A, c);
     bool bad = c.sp.bad;
@@ -528,7 +520,7 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_unit(const PagedArgs A)
     for (c.i = warp; c.i < c.sp.steps; c.i += PG_WARPS) {
         issue(stage == 0 ? PG_STAGES - 1 : stage - 1);
         cp_wait<PG_STAGES - 1>();
-        tile.step(c, ring + stage * S::STAGE, nck, ncv);
+        tile.step(c, chunks + stage * S::STAGE);
         stage = stage + 1 == PG_STAGES ? 0 : stage + 1;
     }
     cp_wait<0>();
@@ -544,12 +536,12 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_unit(const PagedArgs A)
 #pragma unroll
     for (int k = 0; k < S::VCH; k++)
 #pragma unroll
-        for (int e = 0; e < 2 * S::EPC; e += 4) *reinterpret_cast<float4*>(mine + g * D + tile.element(k, e)) = tile.four(k, e, 1.0f);
+        for (int e = 0; e < 2 * S::EPC; e += 4) *reinterpret_cast<float4*>(mine + g * S::DV + tile.element(k, e)) = tile.four(k, e, 1.0f);
     __syncthreads();
     int head0;
     const int heads = tile_heads(A, c.unit, &head0);
-    for (int x = tid; x < heads * D; x += PG_THREADS) {
-        const int h = x / D, d = x - h * D;
+    for (int x = tid; x < heads * S::DV; x += PG_THREADS) {
+        const int h = x / S::DV, d = x - h * S::DV;
         float mm = red[0][h][0];
 #pragma unroll
         for (int w = 1; w < PG_WARPS; w++) mm = fmaxf(mm, red[w][h][0]);
@@ -637,7 +629,8 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_line(const PagedArgs A)
     c.i = static_cast<int>(lo - first - static_cast<long long>(c.unit) * c.sp.steps);
     if (lane == 0) *desc = PagedDesc{lo - c.i, per, c.row, c.unit, c.sp.steps, 0};
 
-    const uint32_t ring = kx::smem_u32(smem) + warp * (PG_STAGES * S::STAGE) + lane * 16;
+    const uint8_t* const chunks = smem + warp * (PG_STAGES * S::STAGE) + lane * 16;
+    const uint32_t ring = kx::smem_u32(chunks);
     const int count = static_cast<int>(hi - lo);
     Cursor<TYPE, D> ahead = c;
     Feed<TYPE, D> feed;
@@ -665,7 +658,7 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_line(const PagedArgs A)
             cp_wait<PG_STAGES - 1>();
             bad = bad || (missing >> stage & 1);
             c.i = i0 + x;
-            tile.step(c, ring + stage * S::STAGE, nck, ncv);
+            tile.step(c, chunks + stage * S::STAGE);
             stage = stage + 1 == PG_STAGES ? 0 : stage + 1;
         }
         bad = __any_sync(FULL, bad);
@@ -696,7 +689,7 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_line(const PagedArgs A)
                 for (int k = 0; k < S::VCH; k++)
 #pragma unroll
                     for (int e = 0; e < 2 * S::EPC; e += 4)
-                        *reinterpret_cast<float4*>(part + g * D + tile.element(k, e)) = tile.four(k, e, 1.0f);
+                        *reinterpret_cast<float4*>(part + g * PG_DMAX + tile.element(k, e)) = tile.four(k, e, 1.0f);
                 if (t == 0) *reinterpret_cast<float2*>(part + PG_HEADS * PG_DMAX + 2 * g) = make_float2(tile.m, tile.l);
             }
         }
@@ -707,7 +700,7 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_line(const PagedArgs A)
 
 // A unit's parts j .. j1 (warps of the line) for head h, every `stride`-th from j + begin on: sum and output (4 elements
 // per lane, in the parts' order) relative to the largest maximum of all parts.
-__device__ __forceinline__ void join_parts(const PagedArgs& A, int j, int j1, int h, int begin, int stride, int D, float4* num, float* den) {
+__device__ __forceinline__ void join_parts(const PagedArgs& A, int j, int j1, int h, int begin, int stride, float4* num, float* den) {
     const int lane = threadIdx.x & 31, d = lane * 4;
     const auto part = [&](int i) { return reinterpret_cast<const float*>(A.ws + part_offset(i, i == j)); };
     float m = -INFINITY;
@@ -722,7 +715,7 @@ __device__ __forceinline__ void join_parts(const PagedArgs& A, int j, int j1, in
         const float* p = part(i);
         const float2 st = __ldcg(reinterpret_cast<const float2*>(p + PG_HEADS * PG_DMAX + 2 * h));
         const float f = kx::ex2(st.x - ms);
-        const float4 v = d < D ? __ldcg(reinterpret_cast<const float4*>(p + h * D + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 v = d < A.c.dv ? __ldcg(reinterpret_cast<const float4*>(p + h * PG_DMAX + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
         *den += f * st.y;
         num->x += f * v.x;
         num->y += f * v.y;
@@ -741,7 +734,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedArgs A, int warps
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     kx::griddep_wait();
     const PagedDesc* desc = reinterpret_cast<const PagedDesc*>(A.ws);
-    const int tasks = (warps - 1) * A.per_chunk, D = A.c.dk <= 64 && A.c.dv <= 64 ? 64 : 128;
+    const int tasks = (warps - 1) * A.per_chunk;
     for (int t0 = blockIdx.x; t0 < tasks; t0 += gridDim.x * 32) {
         if (warp == 0) {
             const int task = t0 + lane * gridDim.x;
@@ -774,7 +767,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedArgs A, int warps
             const PagedDesc ds = desc[j + 1];
             float4 num;
             float den;
-            join_parts(A, j, static_cast<int>((ds.first + ds.steps - 1) / ds.per), h, 0, 1, D, &num, &den);
+            join_parts(A, j, static_cast<int>((ds.first + ds.steps - 1) / ds.per), h, 0, 1, &num, &den);
             const float inv = den == 0.0f ? 0.0f : 1.0f / den;
             if (lane * 4 < A.c.dv) {
                 float* out = output(ds, h) + lane * 4;
@@ -786,7 +779,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedArgs A, int warps
             const PagedDesc ds = desc[j + 1];
             float4 num;
             float den;
-            join_parts(A, j, static_cast<int>((ds.first + ds.steps - 1) / ds.per), h, warp, 8, D, &num, &den);
+            join_parts(A, j, static_cast<int>((ds.first + ds.steps - 1) / ds.per), h, warp, 8, &num, &den);
             *reinterpret_cast<float4*>(&acc[warp][lane * 4]) = num;
             if (lane == 0) sum[warp] = den;
             __syncthreads();
@@ -823,9 +816,15 @@ int launch(const PagedArgs& A, bool split, unsigned grid, cudaStream_t st) {
     return kx::launch_pdl(k_paged_join, dim3(grid), dim3(256), 0, st, A, static_cast<int>(grid * PG_WARPS));
 }
 
+// D: the head dims rounded up to 32; every size runs without a branch inside a step
 template <int TYPE>
 int launch_d(const PagedArgs& A, bool split, unsigned grid, cudaStream_t st) {
-    return A.c.dk <= 64 && A.c.dv <= 64 ? launch<TYPE, 64>(A, split, grid, st) : launch<TYPE, 128>(A, split, grid, st);
+    switch ((std::max(A.c.dk, A.c.dv) + 31) / 32) {
+        case 1: return launch<TYPE, 32>(A, split, grid, st);
+        case 2: return launch<TYPE, 64>(A, split, grid, st);
+        case 3: return launch<TYPE, 96>(A, split, grid, st);
+        default: return launch<TYPE, 128>(A, split, grid, st);
+    }
 }
 
 }  // namespace
