@@ -14,10 +14,9 @@
 //       f32:  tf32 halves, q.k = qh.kh + ql.kh + qh.kl (and p.v likewise), 11 + 11 bits.
 //     That keeps fp32's accuracy (parts lost: below 2^-22 of the operand). A step's p.v is added to the output in
 //     fp32 registers by CUDA-core adds, not carried through the tensor core's truncating accumulation.
-//   * Loads: every lane copies (cp.async, 16 bytes) exactly the chunks that it will use itself as matrix fragments, into
-//     a ring of its own in shared memory: deep prefetch without registers and without barriers. The order of the
-//     reduction axis inside a product is free, so a lane's 16 contiguous bytes serve as they lie; masked keys are
-//     zero-filled and never read.
+//   * Loads: a warp copies (cp.async) its steps' rows into a ring of its own in shared memory: deep prefetch without
+//     registers and without barriers between warps. The order of the reduction axis inside a product is free, so 16
+//     contiguous bytes serve a lane as matrix fragments as they lie; masked keys are zero-filled and never read.
 //   * Work split: the steps of all rows and heads form one line, cut into equal ranges, one per warp (eight warps per
 //     SM); a range may cover several short sequences or a part of a long one. A head whose steps lie in several ranges
 //     is joined by a second launch (programmatic dependent) in the order of the ranges: nothing depends on timing.
@@ -48,9 +47,13 @@ namespace {
 
 constexpr unsigned FULL = 0xFFFFFFFFu;
 constexpr int PG_WARPS = 4, PG_THREADS = PG_WARPS * 32;
-constexpr int PG_STAGES = 3;
+#ifndef PGS
+#define PGS 3
+#define PGB 2
+#endif
+constexpr int PG_STAGES = PGS;
 constexpr int PG_HEADS = 8;       // query heads per tile
-constexpr int PG_MAX_WARPS = 1280;  // of a launch over the line: sizes the workspace
+constexpr int PG_MAX_WARPS = 2048;  // of a launch over the line: sizes the workspace
 constexpr int PG_MIN_STEPS = 4;     // a warp's range is at least this many steps: a part more costs as much as a few
 constexpr int PG_UNIT_STEPS = 24;   // a unit of at most this many steps is one CTA's
 constexpr int PG_DMAX = 128;
@@ -73,7 +76,7 @@ struct PagedArgs {
 struct PagedDesc {
     long long first;  // position of the unit's first step on the line
     long long per;    // steps per warp
-    int row, unit, steps, pad;
+    int row, unit, steps, last;  // last: the warp whose range the unit ends in
 };
 
 // the steps of a row's token: the steps that hold its first tokens, then those of its window
@@ -158,13 +161,16 @@ struct Shape {
     static constexpr int EPC = TYPE == KX_KV_F32 ? 4 : 8;   // elements per 16-byte chunk
     static constexpr int KT = TYPE == KX_KV_F32 ? 1 : 2;    // tiles of 8 keys per step
     static constexpr int KS = 8 * KT;                       // keys per step
-    static constexpr int KCH = D / EPC / 4;                 // K chunks per lane and tile: chunk 4 c + t of key g
-    static constexpr int VK = 2 * KT;                       // V keys per lane: 2 t, 2 t + 1 of each tile
-    static constexpr int VCH = (D / EPC + 7) / 8;           // V chunks per lane and key: chunk 8 c + g
+    static constexpr int CPR = D / EPC;                     // chunks per row
+    static constexpr int PITCH = (CPR + 7) / 8 * 128;       // bytes from row to row in shared memory
+    static constexpr int KCH = CPR / 4;                     // K chunks per lane and tile: chunk 4 c + t
+    static constexpr int VK = 2 * KT;                       // V keys per lane
+    static constexpr int VCH = (CPR + 7) / 8;               // V chunks per lane and key
     static constexpr int NO = VCH * 2 * EPC;                // output elements per lane
     static constexpr int DV = VCH * 8 * EPC;                // a head's outputs, the padding included
-    static constexpr int CH = KT * KCH + VK * VCH;
-    static constexpr int STAGE = CH * 32 * 16;              // bytes per warp and stage
+    static constexpr int CP = KS * CPR / 32;                // chunks that a lane copies, of K and of V
+    static constexpr int TILE = KS * PITCH;                 // K or V of a step
+    static constexpr int STAGE = 2 * TILE;                  // bytes per warp and stage
     static constexpr int QW = D / 4;                        // q elements per lane
     static constexpr int PARTS = TYPE == KX_KV_BF16 ? 3 : 2;
     static constexpr int QP = TYPE == KX_KV_F32 ? QW : QW / 2;  // 32-bit words per part
@@ -220,68 +226,59 @@ struct Feed {
         vb = A.v + static_cast<long>(kvh) * A.c.page * A.c.dv * SZ;
         base = -64;
     }
-    // false: a page that a visible key lies on is not there (its key is then zero-filled, nothing is read)
+    // Rows (keys) of PITCH bytes, chunk x of row r at place x ^ (r & 7): eight lanes that read the same chunk of eight
+    // rows, or four chunks of rows r and r + 4, meet no bank twice. The lanes copy a step's rows in order, so that a
+    // request is 512 contiguous bytes (lanes that copied just what they use themselves asked for 64 bytes of 8 rows:
+    // no barrier, but 4.7 TB/s where this reads at XX). false: a page that a visible key lies on is not there (its key
+    // is then zero-filled, nothing is read). Values of rows that are not seen are zero; chunks behind dk are zero.
     __device__ __forceinline__ bool issue(const PagedArgs& A, const Cursor<TYPE, D>& c, uint32_t dst, int nck, int ncv, int shift) {
-        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, first = c.first_key();
+        const int lane = threadIdx.x & 31, first = c.first_key();
         if ((first >> shift) < base || ((first + S::KS - 1) >> shift) >= base + 32) {
             base = first >> shift;
             ids = base + lane <= (c.sp.len - 1) >> shift ? __ldcg(table + base + lane) : 0;
         }
-        if (A.c.page >= S::KS && c.whole()) {  // one page, every key seen: one base address for K and one for V
-            const int p = __shfl_sync(FULL, ids, (first >> shift) - base);
-            if (p >= 0 && p < A.c.n_pages) {
-                const int slot = first & (A.c.page - 1);
-                const char* ks = kb + p * A.c.k_page * SZ + static_cast<long>((slot + g) * nck + t) * 16;
-                const char* vs = vb + p * A.c.v_page * SZ + static_cast<long>((slot + 2 * t) * ncv + g) * 16;
+        const bool one = A.c.page >= S::KS && c.whole();  // one page, every key seen
+        const int p0 = __shfl_sync(FULL, ids, (first >> shift) - base);
+        if (one && p0 >= 0 && p0 < A.c.n_pages) {
+            const int slot = first & (A.c.page - 1);
+            const char* ks = kb + p0 * A.c.k_page * SZ + static_cast<long>(slot) * nck * 16;
+            const char* vs = vb + p0 * A.c.v_page * SZ + static_cast<long>(slot) * ncv * 16;
 #pragma unroll
-                for (int x = 0; x < S::KCH; x++) {
-                    const bool in = x * 4 + t < nck;
-                    const char* src = in ? ks + x * 64 : A.k;
-#pragma unroll
-                    for (int u = 0; u < S::KT; u++) cp16(dst + (u * S::KCH + x) * 512, src + (in ? u * 128 * nck : 0), in);
-                }
-#pragma unroll
-                for (int x = 0; x < S::VCH; x++) {
-                    const bool in = x * 8 + g < ncv;
-                    const char* src = in ? vs + x * 128 : A.v;
-#pragma unroll
-                    for (int u = 0; u < S::VK; u++)
-                        cp16(dst + (S::KT * S::KCH + u * S::VCH + x) * 512, src + (in ? ((u >> 1) * 8 + (u & 1)) * 16 * ncv : 0), in);
-                }
-                return true;
+            for (int i = 0; i < S::CP; i++) {
+                const int x = i * 32 + lane, r = x / S::CPR, ch = x - r * S::CPR;
+                const bool in = ch < nck;
+                cp16(dst + r * S::PITCH + ((ch ^ (r & 7)) << 4), in ? ks + (r * nck + ch) * 16 : A.k, in);
             }
+#pragma unroll
+            for (int i = 0; i < S::CP; i++) {
+                const int x = i * 32 + lane, r = x / S::CPR, ch = x - r * S::CPR;
+                const bool in = ch < ncv;
+                cp16(dst + S::TILE + r * S::PITCH + ((ch ^ (r & 7)) << 4), in ? vs + (r * ncv + ch) * 16 : A.v, in);
+            }
+            return true;
         }
         bool good = true;
 #pragma unroll
-        for (int u = 0; u < S::KT; u++) {
-            const int j = first + u * 8 + g, p = __shfl_sync(FULL, ids, (j >> shift) - base);
+        for (int i = 0; i < S::CP; i++) {
+            const int x = i * 32 + lane, r = x / S::CPR, ch = x - r * S::CPR, j = first + r;
+            const int p = __shfl_sync(FULL, ids, (j >> shift) - base);
             const bool see = c.visible(j), ok = see && p >= 0 && p < A.c.n_pages;
             good = good && (ok || !see);
-            const char* src = ok ? kb + p * A.c.k_page * SZ + (static_cast<long>(j & (A.c.page - 1)) * nck + t) * 16 : A.k;
-#pragma unroll
-            for (int x = 0; x < S::KCH; x++) {
-                const bool in = ok && x * 4 + t < nck;
-                cp16(dst + (u * S::KCH + x) * 512, in ? src + x * 64 : A.k, in);
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < S::VK; u++) {
-            const int j = first + (u >> 1) * 8 + 2 * t + (u & 1), p = __shfl_sync(FULL, ids, (j >> shift) - base);
-            const bool ok = c.visible(j) && p >= 0 && p < A.c.n_pages;
-            const char* src = ok ? vb + p * A.c.v_page * SZ + (static_cast<long>(j & (A.c.page - 1)) * ncv + g) * 16 : A.v;
-#pragma unroll
-            for (int x = 0; x < S::VCH; x++) {
-                const bool in = ok && x * 8 + g < ncv;
-                cp16(dst + (S::KT * S::KCH + u * S::VCH + x) * 512, in ? src + x * 128 : A.v, in);
-            }
+            const long slot = j & (A.c.page - 1);
+            const uint32_t to = dst + r * S::PITCH + ((ch ^ (r & 7)) << 4);
+            const bool ik = ok && ch < nck, iv = ok && ch < ncv;
+            cp16(to, ik ? kb + p * A.c.k_page * SZ + (slot * nck + ch) * 16 : A.k, ik);
+            cp16(to + S::TILE, iv ? vb + p * A.c.v_page * SZ + (slot * ncv + ch) * 16 : A.v, iv);
         }
         return good;
     }
 };
 
 // One tile of query heads against the cache: q's parts, and the running maximum (in base 2), sum and output. Lane
-// (g, t) holds head g; after the last step its sum is that of its own columns only, and its outputs are the elements
-// 8 EPC c + 2 EPC t + e (o[2 EPC c + e], e < 2 EPC) of the head.
+// (g, t) holds head g; after the last step its sum is that of its own columns only, and its outputs o[2 EPC c + e] are
+// the elements e of chunk 8 c + t (e < EPC) and e - EPC of chunk 8 c + t + 4 of the head.
+// Column n of a tile's scores is the key in row (n >> 1) + 4 (n & 1) of its eight (a lane's columns 2 t and 2 t + 1:
+// rows t and t + 4), and lane g reads its values in chunk (g >> 1) + 4 (g & 1) of eight: the orders without conflicts.
 template <int TYPE, int D>
 struct Tile {
     using S = Shape<TYPE, D>;
@@ -345,9 +342,11 @@ struct Tile {
         l = 0.0f;
     }
 
-    // a step whose chunks lie at src in shared memory
+    // a step whose rows lie at src in shared memory
     __device__ __forceinline__ void step(const Cursor<TYPE, D>& c, const uint8_t* src) {
-        const int t = threadIdx.x & 3;
+        const int g = threadIdx.x >> 2 & 7, t = threadIdx.x & 3, perm = (g >> 1) | (g & 1) << 2;
+        const uint8_t* krow = src + perm * S::PITCH;
+        const int kch[2] = {(t ^ (perm & 3) | (perm & 4)) << 4, (t ^ (perm & 3) | (~perm & 4)) << 4};
         // scores: rows 0-7 and 8-15 of the tile are the products of q's parts
         float s[2 * S::KT];
 #pragma unroll
@@ -356,7 +355,7 @@ struct Tile {
 #pragma unroll
             for (int k = 0; k < S::KCH; k++) {
                 float(&d)[4] = dd[k & 1];
-                const uint4 kv = *reinterpret_cast<const uint4*>(src + (u * S::KCH + k) * 512);
+                const uint4 kv = *reinterpret_cast<const uint4*>(krow + u * 8 * S::PITCH + (k >> 1) * 128 + kch[k & 1]);
                 const int x = k * 4;
                 if constexpr (TYPE == KX_KV_F32) {
                     const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
@@ -381,10 +380,10 @@ struct Tile {
             s[2 * u + 1] = ((dd[0][1] + dd[1][1]) + (dd[0][3] + dd[1][3])) * qscale;
         }
         if (!c.whole()) {
-            const int j = c.first_key() + 2 * t;
+            const int j = c.first_key() + t;
 #pragma unroll
             for (int e = 0; e < 2 * S::KT; e++)
-                if (!c.visible(j + (e >> 1) * 8 + (e & 1))) s[e] = -INFINITY;
+                if (!c.visible(j + e * 4)) s[e] = -INFINITY;
         }
         float mx = s[0];
 #pragma unroll
@@ -406,14 +405,16 @@ struct Tile {
             p[e] = kx::ex2(s[e] - (safe - off));
             l += p[e];
         }
-        // p.v: column 2 t (2 t + 1) of n-tile (k, e) is element e of chunk 8 k + 2 t (+ 1)
-        const uint8_t* vsrc = src + S::KT * S::KCH * 512;
+        // p.v: column 2 t (2 t + 1) of n-tile (k, e) is element e of chunk 8 k + t (+ 4); row t + 4 x of the step is x-th
+        const uint8_t* vrow = src + S::TILE + t * S::PITCH;
+        const int vch[2] = {(perm ^ t) << 4, (perm ^ t ^ 4) << 4};
+        const auto values = [&](int x, int k) { return *reinterpret_cast<const uint4*>(vrow + x * 4 * S::PITCH + k * 128 + vch[x & 1]); };
         if constexpr (TYPE == KX_KV_F32) {
             float q0, q1;
             const uint32_t h0 = tf32_of(p[0], &q0), h1 = tf32_of(p[1], &q1);
 #pragma unroll
             for (int k = 0; k < S::VCH; k++) {
-                const uint4 va = *reinterpret_cast<const uint4*>(vsrc + k * 512), vb = *reinterpret_cast<const uint4*>(vsrc + (S::VCH + k) * 512);
+                const uint4 va = values(0, k), vb = values(1, k);
                 const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -440,7 +441,7 @@ struct Tile {
                 uint32_t w[4][4];
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(vsrc + (u * S::VCH + k) * 512);
+                    const uint4 x = values(u, k);
                     w[u][0] = x.x, w[u][1] = x.y, w[u][2] = x.z, w[u][3] = x.w;
                 }
 #pragma unroll
@@ -467,7 +468,9 @@ struct Tile {
         if (bad) l = NAN;
     }
     // outputs e .. e + 3 of chunk group k: element d of the head
-    __device__ __forceinline__ static int element(int k, int e) { return k * 8 * S::EPC + (threadIdx.x & 3) * 2 * S::EPC + e; }
+    __device__ __forceinline__ static int element(int k, int e) {
+        return (k * 8 + (threadIdx.x & 3)) * S::EPC + (e < S::EPC ? e : e + 3 * S::EPC);
+    }
     __device__ __forceinline__ float4 four(int k, int e, float f) const {
         const float* x = o + k * 2 * S::EPC + e;
         return make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
@@ -487,7 +490,7 @@ __device__ __forceinline__ int tile_heads(const PagedArgs& A, int unit, int* hea
 
 // Short sequences: one CTA per unit, its warps take every fourth step and meet in shared memory.
 template <int TYPE, int D>
-__global__ void __launch_bounds__(PG_THREADS, 2) k_paged_unit(const PagedArgs A) {
+__global__ void __launch_bounds__(PG_THREADS, PGB) k_paged_unit(const PagedArgs A) {
     using S = Shape<TYPE, D>;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float red[PG_WARPS][PG_HEADS][2];
@@ -500,8 +503,8 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_unit(const PagedArgs A)
     c.unit = blockIdx.x - c.row * units;
     c.sp = span_of<S::KS>(A, c.row, &c.slot);
     if (c.sp.steps == 0) return;
-    const uint8_t* const chunks = smem + warp * (PG_STAGES * S::STAGE) + lane * 16;
-    const uint32_t ring = kx::smem_u32(chunks);
+    const uint8_t* const rows = smem + warp * (PG_STAGES * S::STAGE);
+    const uint32_t ring = kx::smem_u32(rows);
     Feed<TYPE, D> feed;
     feed.unit(A, c);
     bool bad = c.sp.bad;
@@ -518,9 +521,11 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_unit(const PagedArgs A)
     tile.start(A, c);
     int stage = 0;
     for (c.i = warp; c.i < c.sp.steps; c.i += PG_WARPS) {
+        __syncwarp();  // every lane has read the rows of the step before
         issue(stage == 0 ? PG_STAGES - 1 : stage - 1);
         cp_wait<PG_STAGES - 1>();
-        tile.step(c, chunks + stage * S::STAGE);
+        __syncwarp();  // every lane's copies of this step are there
+        tile.step(c, rows + stage * S::STAGE);
         stage = stage + 1 == PG_STAGES ? 0 : stage + 1;
     }
     cp_wait<0>();
@@ -560,7 +565,7 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_unit(const PagedArgs A)
 // Warp w of the launch takes the steps [w per, (w + 1) per) of the line, whatever units they belong to; the loads run
 // ahead of the products across the units' ends.
 template <int TYPE, int D>
-__global__ void __launch_bounds__(PG_THREADS, 2) k_paged_line(const PagedArgs A) {
+__global__ void __launch_bounds__(PG_THREADS, PGB) k_paged_line(const PagedArgs A) {
     using S = Shape<TYPE, D>;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ long long upto[PG_THREADS];
@@ -627,10 +632,11 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_line(const PagedArgs A)
     c.sp = span_of<S::KS>(A, c.row, &c.slot);
     c.unit = static_cast<int>((lo - first) / c.sp.steps);
     c.i = static_cast<int>(lo - first - static_cast<long long>(c.unit) * c.sp.steps);
-    if (lane == 0) *desc = PagedDesc{lo - c.i, per, c.row, c.unit, c.sp.steps, 0};
+    if (lane == 0)
+        *desc = PagedDesc{lo - c.i, per, c.row, c.unit, c.sp.steps, static_cast<int>((lo - c.i + c.sp.steps - 1) / per)};
 
-    const uint8_t* const chunks = smem + warp * (PG_STAGES * S::STAGE) + lane * 16;
-    const uint32_t ring = kx::smem_u32(chunks);
+    const uint8_t* const rows = smem + warp * (PG_STAGES * S::STAGE);
+    const uint32_t ring = kx::smem_u32(rows);
     const int count = static_cast<int>(hi - lo);
     Cursor<TYPE, D> ahead = c;
     Feed<TYPE, D> feed;
@@ -654,11 +660,13 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_line(const PagedArgs A)
         bool bad = c.sp.bad;
         tile.start(A, c);
         for (int x = 0; x < steps; x++) {
+            __syncwarp();  // every lane has read the rows of the step before
             issue(stage == 0 ? PG_STAGES - 1 : stage - 1);
             cp_wait<PG_STAGES - 1>();
+            __syncwarp();  // every lane's copies of this step are there
             bad = bad || (missing >> stage & 1);
             c.i = i0 + x;
-            tile.step(c, chunks + stage * S::STAGE);
+            tile.step(c, rows + stage * S::STAGE);
             stage = stage + 1 == PG_STAGES ? 0 : stage + 1;
         }
         bad = __any_sync(FULL, bad);
@@ -698,29 +706,45 @@ __global__ void __launch_bounds__(PG_THREADS, 2) k_paged_line(const PagedArgs A)
     }
 }
 
-// A unit's parts j .. j1 (warps of the line) for head h, every `stride`-th from j + begin on: sum and output (4 elements
-// per lane, in the parts' order) relative to the largest maximum of all parts.
-__device__ __forceinline__ void join_parts(const PagedArgs& A, int j, int j1, int h, int begin, int stride, float4* num, float* den) {
+// A unit's parts j .. j1 (warps of the line) for head h, every STRIDE-th from j + begin on: sum and output (4 elements
+// per lane, in the parts' order) relative to the largest maximum of all parts. Eight parts' loads at a time: the loop
+// is a chain of L2 round trips otherwise.
+template <int STRIDE>
+__device__ __forceinline__ void join_parts(const PagedArgs& A, int j, int j1, int h, int begin, float4* num, float* den) {
     const int lane = threadIdx.x & 31, d = lane * 4;
     const auto part = [&](int i) { return reinterpret_cast<const float*>(A.ws + part_offset(i, i == j)); };
+    constexpr int AT = PG_HEADS * PG_DMAX;
     float m = -INFINITY;
-    for (int i = j + lane; i <= j1; i += 32) m = fmaxf(m, __ldcg(part(i) + PG_HEADS * PG_DMAX + 2 * h));
+    for (int i = j + lane; i <= j1; i += 128) {
+        float x[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) x[u] = i + 32 * u <= j1 ? __ldcg(part(i + 32 * u) + AT + 2 * h) : -INFINITY;
+        m = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), m);
+    }
 #pragma unroll
     for (int z = 16; z; z >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, z));
     const float ms = m == -INFINITY ? 0.0f : m;
     *num = make_float4(0.f, 0.f, 0.f, 0.f);
     *den = 0.0f;
-#pragma unroll 4
-    for (int i = j + begin; i <= j1; i += stride) {
-        const float* p = part(i);
-        const float2 st = __ldcg(reinterpret_cast<const float2*>(p + PG_HEADS * PG_DMAX + 2 * h));
-        const float f = kx::ex2(st.x - ms);
-        const float4 v = d < A.c.dv ? __ldcg(reinterpret_cast<const float4*>(p + h * PG_DMAX + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        *den += f * st.y;
-        num->x += f * v.x;
-        num->y += f * v.y;
-        num->z += f * v.z;
-        num->w += f * v.w;
+    for (int i = j + begin; i <= j1; i += 8 * STRIDE) {
+        float4 v[8];
+        float2 st[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const bool in = i + u * STRIDE <= j1;
+            const float* p = part(in ? i + u * STRIDE : i);
+            st[u] = in ? __ldcg(reinterpret_cast<const float2*>(p + AT + 2 * h)) : make_float2(-INFINITY, 0.0f);
+            v[u] = in && d < A.c.dv ? __ldcg(reinterpret_cast<const float4*>(p + h * PG_DMAX + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const float f = kx::ex2(st[u].x - ms);
+            *den += f * st[u].y;
+            num->x += f * v[u].x;
+            num->y += f * v[u].y;
+            num->z += f * v[u].z;
+            num->w += f * v[u].w;
+        }
     }
 }
 
@@ -742,11 +766,11 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedArgs A, int warps
             if (task < tasks) {
                 const int j = task / A.per_chunk, h = task - j * A.per_chunk;
                 const long long first = __ldcg(&desc[j + 1].first), per = __ldcg(&desc[j + 1].per);
-                const int row = __ldcg(&desc[j + 1].row), unit = __ldcg(&desc[j + 1].unit), steps = __ldcg(&desc[j + 1].steps);
+                const int row = __ldcg(&desc[j + 1].row), unit = __ldcg(&desc[j + 1].unit), last = __ldcg(&desc[j + 1].last);
                 if (row >= 0) {
                     int head0;
                     hit = first >= j * per && first < (j + 1) * per && h < tile_heads(A, unit, &head0);
-                    many = first + steps > (j + 16) * per;
+                    many = last >= j + 16;
                 }
             }
 #pragma unroll
@@ -767,7 +791,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedArgs A, int warps
             const PagedDesc ds = desc[j + 1];
             float4 num;
             float den;
-            join_parts(A, j, static_cast<int>((ds.first + ds.steps - 1) / ds.per), h, 0, 1, &num, &den);
+            join_parts<1>(A, j, ds.last, h, 0, &num, &den);
             const float inv = den == 0.0f ? 0.0f : 1.0f / den;
             if (lane * 4 < A.c.dv) {
                 float* out = output(ds, h) + lane * 4;
@@ -779,7 +803,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedArgs A, int warps
             const PagedDesc ds = desc[j + 1];
             float4 num;
             float den;
-            join_parts(A, j, static_cast<int>((ds.first + ds.steps - 1) / ds.per), h, warp, 8, &num, &den);
+            join_parts<8>(A, j, ds.last, h, warp, &num, &den);
             *reinterpret_cast<float4*>(&acc[warp][lane * 4]) = num;
             if (lane == 0) sum[warp] = den;
             __syncthreads();
@@ -877,7 +901,7 @@ int kx_attention_paged(const kx_kv* c, int layer, const float* q, int ldq, int H
     long keys = static_cast<long>(c->max_pages) * c->page;
     if (window > 0) keys = std::min(keys, static_cast<long>(window) + sinks + 2 * ks);
     const bool split = (keys + ks - 1) / ks > PG_UNIT_STEPS;
-    const unsigned grid = split ? std::min(2 * sms, PG_MAX_WARPS / PG_WARPS) : static_cast<unsigned>(units);
+    const unsigned grid = split ? std::min(PGB * sms, PG_MAX_WARPS / PG_WARPS) : static_cast<unsigned>(units);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (c->type == KX_KV_F32) return launch_d<KX_KV_F32>(A, split, grid, st);
     if (c->type == KX_KV_F16) return launch_d<KX_KV_F16>(A, split, grid, st);
