@@ -20,8 +20,8 @@
 //   * Work split: the steps of all rows and heads form one line, cut into equal ranges, one per warp (eight warps per
 //     SM); a range may cover several short sequences or a part of a long one. A head whose steps lie in several ranges
 //     is joined by a second launch (programmatic dependent) in the order of the ranges: nothing depends on timing.
-//     (One range per CTA, its warps meeting in shared memory at every unit, took 73 us where this takes XX: a CTA
-//     that got many short sequences paid the meeting for each.)
+//     (One range per CTA, its warps meeting in shared memory at every unit, took 80 us for 32 ragged rows of which many
+//     are short, this takes 23: the CTA that got the short ones paid the meeting for each.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -47,14 +47,14 @@ namespace {
 
 constexpr unsigned FULL = 0xFFFFFFFFu;
 constexpr int PG_WARPS = 4, PG_THREADS = PG_WARPS * 32;
-#ifndef PGS
-#define PGS 3
-#define PGB 2
-#endif
-constexpr int PG_STAGES = PGS;
+constexpr int PG_STAGES = 3;
+constexpr int PG_CTAS = 2;        // per SM (three, with registers for each, measured up to 10 % slower)
 constexpr int PG_HEADS = 8;       // query heads per tile
-constexpr int PG_MAX_WARPS = 2048;  // of a launch over the line: sizes the workspace
+constexpr int PG_MAX_WARPS = 1280;  // of a launch over the line: sizes the workspace
 constexpr int PG_MIN_STEPS = 4;     // a warp's range is at least this many steps: a part more costs as much as a few
+// a unit's place on the line before its steps: its q, its output (32 ragged bf16 rows: 26.7 us with 1, 24.7 with 3,
+// 27.7 with 6)
+constexpr int PG_UNIT_COST = 3;
 constexpr int PG_UNIT_STEPS = 24;   // a unit of at most this many steps is one CTA's
 constexpr int PG_DMAX = 128;
 
@@ -75,8 +75,8 @@ struct PagedArgs {
 // what a warp's range begins with: written by the main launch, read by the join
 struct PagedDesc {
     long long first;  // position of the unit's first step on the line
-    long long per;    // steps per warp
-    int row, unit, steps, last;  // last: the warp whose range the unit ends in
+    long long per;    // length of a range
+    int row, unit, last, pad;  // last: the warp whose range the unit ends in
 };
 
 // the steps of a row's token: the steps that hold its first tokens, then those of its window
@@ -130,6 +130,14 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]));
 }
 
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<uint64_t&>(r))
+        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+    return r;
+}
+
 // two fp32 values as PARTS pairs of the 16-bit type, the value = the sum of its parts up to the last one's rounding
 template <int TYPE>
 __device__ __forceinline__ uint32_t pack2(float a, float b, float* ra, float* rb) {
@@ -168,7 +176,6 @@ struct Shape {
     static constexpr int VCH = (CPR + 7) / 8;               // V chunks per lane and key
     static constexpr int NO = VCH * 2 * EPC;                // output elements per lane
     static constexpr int DV = VCH * 8 * EPC;                // a head's outputs, the padding included
-    static constexpr int CP = KS * CPR / 32;                // chunks that a lane copies, of K and of V
     static constexpr int TILE = KS * PITCH;                 // K or V of a step
     static constexpr int STAGE = 2 * TILE;                  // bytes per warp and stage
     static constexpr int QW = D / 4;                        // q elements per lane
@@ -184,6 +191,7 @@ struct Cursor {
     using S = Shape<TYPE, D>;
     Span sp;
     int row, slot, unit, i;
+    long long pos;  // on the line
 
     __device__ __forceinline__ void seek_row(const PagedArgs& A, int r) {  // rows that are left alone have no steps
         do {
@@ -191,15 +199,16 @@ struct Cursor {
             sp = span_of<S::KS>(A, row, &slot);
         } while (sp.steps == 0);
     }
-    // the next step; false: it is another unit's. Not called at the end of the line.
-    __device__ __forceinline__ bool next(const PagedArgs& A, int units) {
-        if (++i < sp.steps) return true;
+    // to the first step of the next unit, or of none if that lies at `end` or behind it
+    __device__ __forceinline__ bool next_unit(const PagedArgs& A, int units, long long end) {
+        pos += sp.steps - i + PG_UNIT_COST;
+        if (pos >= end) return false;
         i = 0;
         if (++unit == units) {
             unit = 0;
             seek_row(A, row + 1);
         }
-        return false;
+        return true;
     }
     __device__ __forceinline__ int first_key() const { return (i < sp.na ? i : i - sp.na + sp.b0) * S::KS; }
     // every key of the step is seen
@@ -227,63 +236,69 @@ struct Feed {
         base = -64;
     }
     // Rows (keys) of PITCH bytes, chunk x of row r at place x ^ (r & 7): eight lanes that read the same chunk of eight
-    // rows, or four chunks of rows r and r + 4, meet no bank twice. The lanes copy a step's rows in order, so that a
-    // request is 512 contiguous bytes (lanes that copied just what they use themselves asked for 64 bytes of 8 rows:
-    // no barrier, but 4.7 TB/s where this reads at XX). false: a page that a visible key lies on is not there (its key
-    // is then zero-filled, nothing is read). Values of rows that are not seen are zero; chunks behind dk are zero.
+    // rows, or four chunks of rows r and r + 4, meet no bank twice. Eight lanes copy 128 contiguous bytes of a row (lanes
+    // that copied just what they use themselves asked for 64 bytes at a time: no barrier, but 4.7 TB/s where this reads
+    // at 5.8); lane offsets are the same in every step. Chunks behind a row's end are left as they are (zero_pads); rows
+    // that are not seen become zero. false: a page that a visible key lies on is not there; its row is zero, too.
     __device__ __forceinline__ bool issue(const PagedArgs& A, const Cursor<TYPE, D>& c, uint32_t dst, int nck, int ncv, int shift) {
-        const int lane = threadIdx.x & 31, first = c.first_key();
+        const int lane = threadIdx.x & 31, first = c.first_key(), lr = lane >> 3, lc = lane & 7;
         if ((first >> shift) < base || ((first + S::KS - 1) >> shift) >= base + 32) {
             base = first >> shift;
             ids = base + lane <= (c.sp.len - 1) >> shift ? __ldcg(table + base + lane) : 0;
         }
-        const bool one = A.c.page >= S::KS && c.whole();  // one page, every key seen
+        // rows lr + 4 y, chunks lc + 8 x
+        const uint32_t to[2] = {dst + lr * S::PITCH + ((lc ^ lr) << 4), dst + lr * S::PITCH + ((lc ^ lr ^ 4) << 4)};
         const int p0 = __shfl_sync(FULL, ids, (first >> shift) - base);
-        if (one && p0 >= 0 && p0 < A.c.n_pages) {
-            const int slot = first & (A.c.page - 1);
-            const char* ks = kb + p0 * A.c.k_page * SZ + static_cast<long>(slot) * nck * 16;
-            const char* vs = vb + p0 * A.c.v_page * SZ + static_cast<long>(slot) * ncv * 16;
+        if (A.c.page >= S::KS && c.whole() && p0 >= 0 && p0 < A.c.n_pages) {  // one page, every key seen
+            const int slot = (first & (A.c.page - 1)) + lr;
+            const char* ks = kb + p0 * A.c.k_page * SZ + (static_cast<long>(slot) * nck + lc) * 16;
+            const char* vs = vb + p0 * A.c.v_page * SZ + (static_cast<long>(slot) * ncv + lc) * 16;
 #pragma unroll
-            for (int i = 0; i < S::CP; i++) {
-                const int x = i * 32 + lane, r = x / S::CPR, ch = x - r * S::CPR;
-                const bool in = ch < nck;
-                cp16(dst + r * S::PITCH + ((ch ^ (r & 7)) << 4), in ? ks + (r * nck + ch) * 16 : A.k, in);
-            }
+            for (int y = 0; y < S::KS / 4; y++, ks += 64 * nck)
 #pragma unroll
-            for (int i = 0; i < S::CP; i++) {
-                const int x = i * 32 + lane, r = x / S::CPR, ch = x - r * S::CPR;
-                const bool in = ch < ncv;
-                cp16(dst + S::TILE + r * S::PITCH + ((ch ^ (r & 7)) << 4), in ? vs + (r * ncv + ch) * 16 : A.v, in);
-            }
+                for (int x = 0; x < S::VCH; x++)
+                    if (lc + 8 * x < nck) cp16(to[y & 1] + y * 4 * S::PITCH + x * 128, ks + x * 128, true);
+#pragma unroll
+            for (int y = 0; y < S::KS / 4; y++, vs += 64 * ncv)
+#pragma unroll
+                for (int x = 0; x < S::VCH; x++)
+                    if (lc + 8 * x < ncv) cp16(to[y & 1] + S::TILE + y * 4 * S::PITCH + x * 128, vs + x * 128, true);
             return true;
         }
         bool good = true;
 #pragma unroll
-        for (int i = 0; i < S::CP; i++) {
-            const int x = i * 32 + lane, r = x / S::CPR, ch = x - r * S::CPR, j = first + r;
-            const int p = __shfl_sync(FULL, ids, (j >> shift) - base);
+        for (int y = 0; y < S::KS / 4; y++) {
+            const int j = first + lr + 4 * y, p = __shfl_sync(FULL, ids, (j >> shift) - base);
             const bool see = c.visible(j), ok = see && p >= 0 && p < A.c.n_pages;
             good = good && (ok || !see);
             const long slot = j & (A.c.page - 1);
-            const uint32_t to = dst + r * S::PITCH + ((ch ^ (r & 7)) << 4);
-            const bool ik = ok && ch < nck, iv = ok && ch < ncv;
-            cp16(to, ik ? kb + p * A.c.k_page * SZ + (slot * nck + ch) * 16 : A.k, ik);
-            cp16(to + S::TILE, iv ? vb + p * A.c.v_page * SZ + (slot * ncv + ch) * 16 : A.v, iv);
+            const char* ks = ok ? kb + p * A.c.k_page * SZ + (slot * nck + lc) * 16 : A.k;
+            const char* vs = ok ? vb + p * A.c.v_page * SZ + (slot * ncv + lc) * 16 : A.v;
+#pragma unroll
+            for (int x = 0; x < S::VCH; x++) {
+                if (lc + 8 * x < nck) cp16(to[y & 1] + y * 4 * S::PITCH + x * 128, ok ? ks + x * 128 : A.k, ok);
+                if (lc + 8 * x < ncv) cp16(to[y & 1] + S::TILE + y * 4 * S::PITCH + x * 128, ok ? vs + x * 128 : A.v, ok);
+            }
         }
         return good;
+    }
+    // the chunks behind dk, which no copy writes, count in the scores as zeros
+    __device__ __forceinline__ static void zero_pads(uint8_t* rows, int nck) {
+        if (nck == S::CPR) return;
+        for (int x = (threadIdx.x & 31) * 16; x < PG_STAGES * S::STAGE; x += 512) *reinterpret_cast<uint4*>(rows + x) = make_uint4(0, 0, 0, 0);
+        __syncwarp();
     }
 };
 
 // One tile of query heads against the cache: q's parts, and the running maximum (in base 2), sum and output. Lane
-// (g, t) holds head g; after the last step its sum is that of its own columns only, and its outputs o[2 EPC c + e] are
-// the elements e of chunk 8 c + t (e < EPC) and e - EPC of chunk 8 c + t + 4 of the head.
+// (g, t) holds head g; after the last step its sum is that of its own columns only.
 // Column n of a tile's scores is the key in row (n >> 1) + 4 (n & 1) of its eight (a lane's columns 2 t and 2 t + 1:
 // rows t and t + 4), and lane g reads its values in chunk (g >> 1) + 4 (g & 1) of eight: the orders without conflicts.
 template <int TYPE, int D>
 struct Tile {
     using S = Shape<TYPE, D>;
     uint32_t qp[S::PARTS][S::QP];
-    float o[S::NO];
+    float2 o[S::NO / 2];  // o[EPC c + e]: elements e of chunks 8 c + t and 8 c + t + 4
     float m, l, qscale, off;
 
     // x: the head's q, lane t the elements that its K chunks hold
@@ -337,7 +352,7 @@ struct Tile {
             }
         }
 #pragma unroll
-        for (int k = 0; k < S::NO; k++) o[k] = 0.0f;
+        for (int k = 0; k < S::NO / 2; k++) o[k] = make_float2(0.0f, 0.0f);
         m = -INFINITY;
         l = 0.0f;
     }
@@ -351,10 +366,11 @@ struct Tile {
         float s[2 * S::KT];
 #pragma unroll
         for (int u = 0; u < S::KT; u++) {
-            float dd[2][4] = {};  // two chains of products
+            float dd[4][4] = {};  // chains of products: by even and odd chunk, and the last part's apart
 #pragma unroll
             for (int k = 0; k < S::KCH; k++) {
                 float(&d)[4] = dd[k & 1];
+                float(&f)[4] = dd[2 + (k & 1)];
                 const uint4 kv = *reinterpret_cast<const uint4*>(krow + u * 8 * S::PITCH + (k >> 1) * 128 + kch[k & 1]);
                 const int x = k * 4;
                 if constexpr (TYPE == KX_KV_F32) {
@@ -364,7 +380,7 @@ struct Tile {
                         float l0, l1;
                         const uint32_t h0 = tf32_of(__uint_as_float(w[h]), &l0), h1 = tf32_of(__uint_as_float(w[h + 1]), &l1);
                         mma_tf32(d, qp[0][x + h], qp[1][x + h], qp[0][x + h + 1], qp[1][x + h + 1], h0, h1);
-                        mma_tf32(d, qp[0][x + h], 0, qp[0][x + h + 1], 0, __float_as_uint(l0), __float_as_uint(l1));
+                        mma_tf32(f, qp[0][x + h], 0, qp[0][x + h + 1], 0, __float_as_uint(l0), __float_as_uint(l1));
                     }
                 } else if constexpr (TYPE == KX_KV_F16) {
                     mma_f16(d, qp[0][x], qp[1][x], qp[0][x + 1], qp[1][x + 1], kv.x, kv.y);
@@ -372,12 +388,13 @@ struct Tile {
                 } else {
                     mma_bf16(d, qp[0][x], qp[1][x], qp[0][x + 1], qp[1][x + 1], kv.x, kv.y);
                     mma_bf16(d, qp[0][x + 2], qp[1][x + 2], qp[0][x + 3], qp[1][x + 3], kv.z, kv.w);
-                    mma_bf16(d, qp[2][x], 0, qp[2][x + 1], 0, kv.x, kv.y);
-                    mma_bf16(d, qp[2][x + 2], 0, qp[2][x + 3], 0, kv.z, kv.w);
+                    mma_bf16(f, qp[2][x], 0, qp[2][x + 1], 0, kv.x, kv.y);
+                    mma_bf16(f, qp[2][x + 2], 0, qp[2][x + 3], 0, kv.z, kv.w);
                 }
             }
-            s[2 * u] = ((dd[0][0] + dd[1][0]) + (dd[0][2] + dd[1][2])) * qscale;
-            s[2 * u + 1] = ((dd[0][1] + dd[1][1]) + (dd[0][3] + dd[1][3])) * qscale;
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+                s[2 * u + e] = ((dd[0][e] + dd[1][e]) + ((dd[0][e + 2] + dd[1][e + 2]) + (dd[2][e] + dd[3][e]))) * qscale;
         }
         if (!c.whole()) {
             const int j = c.first_key() + t;
@@ -396,7 +413,7 @@ struct Tile {
             const float alpha = kx::ex2(m - safe);
             l *= alpha;
 #pragma unroll
-            for (int e = 0; e < S::NO; e++) o[e] *= alpha;
+            for (int e = 0; e < S::NO / 2; e++) o[e].x *= alpha, o[e].y *= alpha;
         }
         m = mn;
         float p[2 * S::KT];
@@ -422,8 +439,7 @@ struct Tile {
                     const uint32_t v0 = tf32_of(__uint_as_float(wa[e]), &l0), v1 = tf32_of(__uint_as_float(wb[e]), &l1);
                     mma_tf32(d, h0, 0, h1, 0, __float_as_uint(l0), __float_as_uint(l1));
                     mma_tf32(d, h0, __float_as_uint(q0), h1, __float_as_uint(q1), v0, v1);
-                    o[k * 8 + e] += d[0] + d[2];
-                    o[k * 8 + 4 + e] += d[1] + d[3];
+                    o[k * 4 + e] = add2(o[k * 4 + e], add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])));
                 }
             }
         } else {
@@ -455,8 +471,7 @@ struct Tile {
                         mma_bf16(d, pa[2], 0, pb[2], 0, b0, b1);
                         mma_bf16(d, pa[0], pa[1], pb[0], pb[1], b0, b1);
                     }
-                    o[k * 16 + e] += d[0] + d[2];
-                    o[k * 16 + 8 + e] += d[1] + d[3];
+                    o[k * 8 + e] = add2(o[k * 8 + e], add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])));
                 }
             }
         }
@@ -472,8 +487,9 @@ struct Tile {
         return (k * 8 + (threadIdx.x & 3)) * S::EPC + (e < S::EPC ? e : e + 3 * S::EPC);
     }
     __device__ __forceinline__ float4 four(int k, int e, float f) const {
-        const float* x = o + k * 2 * S::EPC + e;
-        return make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+        const float2* x = o + k * S::EPC + e % S::EPC;
+        return e < S::EPC ? make_float4(x[0].x * f, x[1].x * f, x[2].x * f, x[3].x * f)
+                          : make_float4(x[0].y * f, x[1].y * f, x[2].y * f, x[3].y * f);
     }
 };
 
@@ -490,7 +506,7 @@ __device__ __forceinline__ int tile_heads(const PagedArgs& A, int unit, int* hea
 
 // Short sequences: one CTA per unit, its warps take every fourth step and meet in shared memory.
 template <int TYPE, int D>
-__global__ void __launch_bounds__(PG_THREADS, PGB) k_paged_unit(const PagedArgs A) {
+__global__ void __launch_bounds__(PG_THREADS, PG_CTAS) k_paged_unit(const PagedArgs A) {
     using S = Shape<TYPE, D>;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ float red[PG_WARPS][PG_HEADS][2];
@@ -503,8 +519,9 @@ __global__ void __launch_bounds__(PG_THREADS, PGB) k_paged_unit(const PagedArgs 
     c.unit = blockIdx.x - c.row * units;
     c.sp = span_of<S::KS>(A, c.row, &c.slot);
     if (c.sp.steps == 0) return;
-    const uint8_t* const rows = smem + warp * (PG_STAGES * S::STAGE);
+    uint8_t* const rows = smem + warp * (PG_STAGES * S::STAGE);
     const uint32_t ring = kx::smem_u32(rows);
+    Feed<TYPE, D>::zero_pads(rows, nck);
     Feed<TYPE, D> feed;
     feed.unit(A, c);
     bool bad = c.sp.bad;
@@ -565,7 +582,7 @@ __global__ void __launch_bounds__(PG_THREADS, PGB) k_paged_unit(const PagedArgs 
 // Warp w of the launch takes the steps [w per, (w + 1) per) of the line, whatever units they belong to; the loads run
 // ahead of the products across the units' ends.
 template <int TYPE, int D>
-__global__ void __launch_bounds__(PG_THREADS, PGB) k_paged_line(const PagedArgs A) {
+__global__ void __launch_bounds__(PG_THREADS, PG_CTAS) k_paged_line(const PagedArgs A) {
     using S = Shape<TYPE, D>;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ long long upto[PG_THREADS];
@@ -575,11 +592,13 @@ __global__ void __launch_bounds__(PG_THREADS, PGB) k_paged_line(const PagedArgs 
     kx::griddep_wait();
     kx::griddep_launch_dependents();
 
-    // rows r0 .. r0 + PG_THREADS - 1: upto[x] = steps per unit of the rows r0 .. r0 + x; returns the last of them
+    // rows r0 .. r0 + PG_THREADS - 1: upto[x] = a unit's length on the line, summed over the rows r0 .. r0 + x; returns
+    // the last of them
     const auto scan_rows = [&](int r0) {
         int slot;
         const int r = r0 + tid;
         long long v = r < A.n ? span_of<S::KS>(A, r, &slot).steps : 0;
+        if (v > 0) v += PG_UNIT_COST;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const long long u = __shfl_up_sync(FULL, v, d);
@@ -606,7 +625,7 @@ __global__ void __launch_bounds__(PG_THREADS, PGB) k_paged_line(const PagedArgs 
     const long long lo = me * per, hi = min(lo + per, total);
     Cursor<TYPE, D> c;
     c.row = -1;
-    long long first = 0;  // the row's first step on the line
+    long long first = 0;  // where the row begins
     long long before = 0;
     for (int r0 = 0; r0 < A.n; r0 += PG_THREADS) {  // the row that lo lies in
         const long long all = A.n > PG_THREADS ? scan_rows(r0) : total / units;
@@ -625,29 +644,37 @@ __global__ void __launch_bounds__(PG_THREADS, PGB) k_paged_line(const PagedArgs 
         before += all;
     }
     PagedDesc* desc = reinterpret_cast<PagedDesc*>(A.ws) + me;
-    if (c.row < 0) {
+    if (c.row >= 0) {
+        c.sp = span_of<S::KS>(A, c.row, &c.slot);
+        const int length = c.sp.steps + PG_UNIT_COST;
+        c.unit = static_cast<int>((lo - first) / length);
+        first += static_cast<long long>(c.unit) * length + PG_UNIT_COST;  // the unit's first step
+        c.pos = max(lo, first);
+        c.i = static_cast<int>(c.pos - first);
+    }
+    if (c.row < 0 || c.pos >= hi) {
         if (lane == 0) desc->row = -1;
         return;
     }
-    c.sp = span_of<S::KS>(A, c.row, &c.slot);
-    c.unit = static_cast<int>((lo - first) / c.sp.steps);
-    c.i = static_cast<int>(lo - first - static_cast<long long>(c.unit) * c.sp.steps);
-    if (lane == 0)
-        *desc = PagedDesc{lo - c.i, per, c.row, c.unit, c.sp.steps, static_cast<int>((lo - c.i + c.sp.steps - 1) / per)};
+    if (lane == 0) *desc = PagedDesc{first, per, c.row, c.unit, static_cast<int>((first + c.sp.steps - 1) / per), 0};
 
-    const uint8_t* const rows = smem + warp * (PG_STAGES * S::STAGE);
+    uint8_t* const rows = smem + warp * (PG_STAGES * S::STAGE);
     const uint32_t ring = kx::smem_u32(rows);
-    const int count = static_cast<int>(hi - lo);
+    Feed<TYPE, D>::zero_pads(rows, nck);
     Cursor<TYPE, D> ahead = c;
     Feed<TYPE, D> feed;
     feed.unit(A, ahead);
-    int sent = 0;
     unsigned missing = 0;  // per stage: a page was not there
     const auto issue = [&](int stage) {
-        if (sent < count) {
+        if (ahead.pos < hi) {
             const bool good = feed.issue(A, ahead, ring + stage * S::STAGE, nck, ncv, shift);
             missing = (missing & ~(1u << stage)) | (good ? 0u : 1u << stage);
-            if (++sent < count && !ahead.next(A, units)) feed.unit(A, ahead);
+            if (ahead.i + 1 < ahead.sp.steps) {
+                ahead.i++;
+                ahead.pos++;
+            } else if (ahead.next_unit(A, units, hi)) {
+                feed.unit(A, ahead);
+            }
         }
         cp_commit();
     };
@@ -655,8 +682,8 @@ __global__ void __launch_bounds__(PG_THREADS, PGB) k_paged_line(const PagedArgs 
     for (int s = 0; s < PG_STAGES - 1; s++) issue(s);
     Tile<TYPE, D> tile;
     int stage = 0;
-    for (int done = 0; done < count;) {
-        const int i0 = c.i, steps = min(c.sp.steps - c.i, count - done);
+    do {
+        const int i0 = c.i, steps = static_cast<int>(min(static_cast<long long>(c.sp.steps - c.i), hi - c.pos));
         bool bad = c.sp.bad;
         tile.start(A, c);
         for (int x = 0; x < steps; x++) {
@@ -701,44 +728,39 @@ __global__ void __launch_bounds__(PG_THREADS, PGB) k_paged_line(const PagedArgs 
                 if (t == 0) *reinterpret_cast<float2*>(part + PG_HEADS * PG_DMAX + 2 * g) = make_float2(tile.m, tile.l);
             }
         }
-        done += steps;
-        if (done < count) c.next(A, units);
-    }
+        c.i = i0;
+    } while (c.next_unit(A, units, hi));
 }
 
-// A unit's parts j .. j1 (warps of the line) for head h, every STRIDE-th from j + begin on: sum and output (4 elements
-// per lane, in the parts' order) relative to the largest maximum of all parts. Eight parts' loads at a time: the loop
-// is a chain of L2 round trips otherwise.
+// A unit's parts j .. j1 (warps of the line) for head h, every STRIDE-th from j + begin on: maximum, sum and output (4
+// elements per lane), in the parts' order. Eight parts' loads at a time: the loop is a chain of L2 round trips.
 template <int STRIDE>
-__device__ __forceinline__ void join_parts(const PagedArgs& A, int j, int j1, int h, int begin, float4* num, float* den) {
-    const int lane = threadIdx.x & 31, d = lane * 4;
-    const auto part = [&](int i) { return reinterpret_cast<const float*>(A.ws + part_offset(i, i == j)); };
-    constexpr int AT = PG_HEADS * PG_DMAX;
-    float m = -INFINITY;
-    for (int i = j + lane; i <= j1; i += 128) {
-        float x[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++) x[u] = i + 32 * u <= j1 ? __ldcg(part(i + 32 * u) + AT + 2 * h) : -INFINITY;
-        m = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), m);
-    }
-#pragma unroll
-    for (int z = 16; z; z >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, z));
-    const float ms = m == -INFINITY ? 0.0f : m;
-    *num = make_float4(0.f, 0.f, 0.f, 0.f);
+__device__ __forceinline__ void join_parts(const PagedArgs& A, int j, int j1, int h, int begin, float* m, float* den, float4* num) {
+    const int d = (threadIdx.x & 31) * 4;
+    *m = -INFINITY;
     *den = 0.0f;
+    *num = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int i = j + begin; i <= j1; i += 8 * STRIDE) {
         float4 v[8];
         float2 st[8];
 #pragma unroll
         for (int u = 0; u < 8; u++) {
-            const bool in = i + u * STRIDE <= j1;
-            const float* p = part(in ? i + u * STRIDE : i);
-            st[u] = in ? __ldcg(reinterpret_cast<const float2*>(p + AT + 2 * h)) : make_float2(-INFINITY, 0.0f);
+            const int at = i + u * STRIDE;
+            const bool in = at <= j1;
+            const float* p = reinterpret_cast<const float*>(A.ws + part_offset(in ? at : i, (in ? at : i) == j));
+            st[u] = in ? __ldcg(reinterpret_cast<const float2*>(p + PG_HEADS * PG_DMAX + 2 * h)) : make_float2(-INFINITY, 0.0f);
             v[u] = in && d < A.c.dv ? __ldcg(reinterpret_cast<const float4*>(p + h * PG_DMAX + d)) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
+        float top = *m;
+#pragma unroll
+        for (int u = 0; u < 8; u++) top = fmaxf(top, st[u].x);
+        const float safe = top == -INFINITY ? 0.0f : top, back = kx::ex2(*m - safe);
+        *m = top;
+        *den *= back;
+        num->x *= back, num->y *= back, num->z *= back, num->w *= back;
 #pragma unroll
         for (int u = 0; u < 8; u++) {
-            const float f = kx::ex2(st[u].x - ms);
+            const float f = kx::ex2(st[u].x - safe);
             *den += f * st[u].y;
             num->x += f * v[u].x;
             num->y += f * v[u].y;
@@ -753,8 +775,9 @@ __device__ __forceinline__ void join_parts(const PagedArgs& A, int j, int j1, in
 // every eighth part, then the warps' sums in order.
 __global__ void __launch_bounds__(256) k_paged_join(const PagedArgs A, int warps) {
     __shared__ float acc[8][PG_DMAX];
-    __shared__ float sum[8];
-    __shared__ int todo[2][32], n_todo[2];  // few parts, many parts
+    __shared__ float sum[8], top[8];
+    __shared__ int4 todo[2][32];  // few parts, many parts: j, last part, head of the tile, head of the row
+    __shared__ int todo_row[2][32], n_todo[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     kx::griddep_wait();
     const PagedDesc* desc = reinterpret_cast<const PagedDesc*>(A.ws);
@@ -763,58 +786,64 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedArgs A, int warps
         if (warp == 0) {
             const int task = t0 + lane * gridDim.x;
             bool hit = false, many = false;
+            int4 what = make_int4(0, 0, 0, 0);
+            int row = -1;
             if (task < tasks) {
                 const int j = task / A.per_chunk, h = task - j * A.per_chunk;
-                const long long first = __ldcg(&desc[j + 1].first), per = __ldcg(&desc[j + 1].per);
-                const int row = __ldcg(&desc[j + 1].row), unit = __ldcg(&desc[j + 1].unit), last = __ldcg(&desc[j + 1].last);
-                if (row >= 0) {
+                const longlong2 line = __ldcg(reinterpret_cast<const longlong2*>(&desc[j + 1].first));
+                const int4 unit = __ldcg(reinterpret_cast<const int4*>(&desc[j + 1].row));
+                if (unit.x >= 0) {
                     int head0;
-                    hit = first >= j * per && first < (j + 1) * per && h < tile_heads(A, unit, &head0);
-                    many = last >= j + 16;
+                    hit = line.x >= j * line.y && line.x < (j + 1) * line.y && h < tile_heads(A, unit.y, &head0);
+                    many = unit.z >= j + 16;
+                    what = make_int4(j, unit.z, h, head0 + h);
+                    row = unit.x;
                 }
             }
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-                const unsigned hits = __ballot_sync(FULL, hit && many == (x == 1));
-                if (hit && many == (x == 1)) todo[x][__popc(hits & ((1u << lane) - 1))] = task;
+                const bool mine = hit && many == (x == 1);
+                const unsigned hits = __ballot_sync(FULL, mine);
+                if (mine) {
+                    todo[x][__popc(hits & ((1u << lane) - 1))] = what;
+                    todo_row[x][__popc(hits & ((1u << lane) - 1))] = row;
+                }
                 if (lane == 0) n_todo[x] = __popc(hits);
             }
         }
         __syncthreads();
-        const auto output = [&](const PagedDesc& ds, int h) {
-            int head0;
-            tile_heads(A, ds.unit, &head0);
-            return A.ctx + static_cast<long>(ds.row) * A.ldc + static_cast<long>(head0 + h) * A.c.dv;
-        };
+        float m, den;
+        float4 num;
         for (int x = warp; x < n_todo[0]; x += 8) {
-            const int j = todo[0][x] / A.per_chunk, h = todo[0][x] - j * A.per_chunk;
-            const PagedDesc ds = desc[j + 1];
-            float4 num;
-            float den;
-            join_parts<1>(A, j, ds.last, h, 0, &num, &den);
+            const int4 w = todo[0][x];
+            join_parts<1>(A, w.x, w.y, w.z, 0, &m, &den, &num);
             const float inv = den == 0.0f ? 0.0f : 1.0f / den;
             if (lane * 4 < A.c.dv) {
-                float* out = output(ds, h) + lane * 4;
+                float* out = A.ctx + static_cast<long>(todo_row[0][x]) * A.ldc + static_cast<long>(w.w) * A.c.dv + lane * 4;
                 out[0] = num.x * inv, out[1] = num.y * inv, out[2] = num.z * inv, out[3] = num.w * inv;
             }
         }
         for (int x = 0; x < n_todo[1]; x++) {
-            const int j = todo[1][x] / A.per_chunk, h = todo[1][x] - j * A.per_chunk;
-            const PagedDesc ds = desc[j + 1];
-            float4 num;
-            float den;
-            join_parts<8>(A, j, ds.last, h, warp, &num, &den);
+            const int4 w = todo[1][x];
+            join_parts<8>(A, w.x, w.y, w.z, warp, &m, &den, &num);
             *reinterpret_cast<float4*>(&acc[warp][lane * 4]) = num;
-            if (lane == 0) sum[warp] = den;
+            if (lane == 0) {
+                sum[warp] = den;
+                top[warp] = m;
+            }
             __syncthreads();
             if (tid < A.c.dv) {
-                float n = 0.0f, l = 0.0f;
+                float n = 0.0f, l = 0.0f, all = top[0];
 #pragma unroll
-                for (int w = 0; w < 8; w++) {
-                    n += acc[w][tid];
-                    l += sum[w];
+                for (int z = 1; z < 8; z++) all = fmaxf(all, top[z]);
+                const float safe = all == -INFINITY ? 0.0f : all;
+#pragma unroll
+                for (int z = 0; z < 8; z++) {
+                    const float f = kx::ex2(top[z] - safe);
+                    n += f * acc[z][tid];
+                    l += f * sum[z];
                 }
-                output(ds, h)[tid] = l == 0.0f ? 0.0f : n / l;
+                A.ctx[static_cast<long>(todo_row[1][x]) * A.ldc + static_cast<long>(w.w) * A.c.dv + tid] = l == 0.0f ? 0.0f : n / l;
             }
             __syncthreads();
         }
@@ -901,7 +930,7 @@ int kx_attention_paged(const kx_kv* c, int layer, const float* q, int ldq, int H
     long keys = static_cast<long>(c->max_pages) * c->page;
     if (window > 0) keys = std::min(keys, static_cast<long>(window) + sinks + 2 * ks);
     const bool split = (keys + ks - 1) / ks > PG_UNIT_STEPS;
-    const unsigned grid = split ? std::min(PGB * sms, PG_MAX_WARPS / PG_WARPS) : static_cast<unsigned>(units);
+    const unsigned grid = split ? std::min(PG_CTAS * sms, PG_MAX_WARPS / PG_WARPS) : static_cast<unsigned>(units);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (c->type == KX_KV_F32) return launch_d<KX_KV_F32>(A, split, grid, st);
     if (c->type == KX_KV_F16) return launch_d<KX_KV_F16>(A, split, grid, st);
