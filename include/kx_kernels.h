@@ -328,6 +328,21 @@ KERNIX_API int kx_attention_paged(const kx_kv* c, int layer, const float* q, int
                                   int sinks, float scale, float* ctx, int ldc, void* ws, size_t ws_bytes, int* status,
                                   void* stream);
 
+/* Attention of prompts with a sliding window whose first tokens stay visible (fp32 rows as kx_attention's, but heads that
+ * share keys and values, ragged samples, any length). Sample b has q_len[b] <= Rq query rows b * Rq + i (ldq, H * dk
+ * floats) and k_len[b] <= S key and value rows b * S + j (ldk, Hkv * dk; ldv, Hkv * dv); q_len, k_len: device words, NULL =
+ * Rq, S. Its queries are the last tokens: query i is at position t = k_len - q_len + i and sees key j when j <= t and
+ * (window <= 0 or j > t - window or j < sinks). ctx rows b * Rq + i (ldc, H * dv floats); a row that sees nothing (t < 0)
+ * becomes 0, rows i >= q_len are left as they were; a sample whose lengths are out of range is reported
+ * (KX_STATUS_BAD_REQUEST) and its Rq rows become NaN. Query head h reads key-value head h / (H / Hkv). scale 0 means
+ * 1/sqrt(dk). dk, dv <= 128, H a multiple of Hkv. q, k, v must not overlap ctx or ws. ws: kx_attention_window_ws bytes
+ * of device workspace (0: the arguments are invalid), 128-byte aligned, shared under kx_kv_ws's rules. Key and value
+ * rows that no query of the sample sees do not affect results, whatever they hold. */
+KERNIX_API size_t kx_attention_window_ws(int B, int S, int Hkv, int dk, int dv);
+KERNIX_API int kx_attention_window(const float* q, int ldq, const float* k, int ldk, const float* v, int ldv, float* ctx, int ldc,
+                                   int B, int Rq, int S, int H, int Hkv, int dk, int dv, const int32_t* q_len, const int32_t* k_len,
+                                   int window, int sinks, float scale, void* ws, size_t ws_bytes, int* status, void* stream);
+
 /* y = max(a*x + b, 0), fused multiply-add then max (src/kernix_metal.m:331-338; include/kernix.h:990) */
 KERNIX_API int kx_fma_relu(const float* a, const float* x, const float* b, float* y, size_t n, void* stream);
 

@@ -30,18 +30,11 @@
 #include <cmath>
 #include <cstdint>
 
+#include "kx_act.cuh"
 #include "kx_kernels.h"
 #include "kx_kv.cuh"
 #include "kx_pdl.cuh"
 #include "kx_sm100.cuh"
-
-namespace kx {
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-}  // namespace kx
 
 namespace {
 
@@ -410,7 +403,7 @@ struct Tile {
         const float mn = fmaxf(m, mx);
         const float safe = mn == -INFINITY ? 0.0f : mn;
         if (__any_sync(FULL, mn > m)) {
-            const float alpha = kx::ex2(m - safe);
+            const float alpha = kx::ex2_approx(m - safe);
             l *= alpha;
 #pragma unroll
             for (int e = 0; e < S::NO / 2; e++) o[e].x *= alpha, o[e].y *= alpha;
@@ -419,7 +412,7 @@ struct Tile {
         float p[2 * S::KT];
 #pragma unroll
         for (int e = 0; e < 2 * S::KT; e++) {
-            p[e] = kx::ex2(s[e] - (safe - off));
+            p[e] = kx::ex2_approx(s[e] - (safe - off));
             l += p[e];
         }
         // p.v: column 2 t (2 t + 1) of n-tile (k, e) is element e of chunk 8 k + t (+ 4); row t + 4 x of the step is x-th
@@ -571,7 +564,7 @@ __global__ void __launch_bounds__(PG_THREADS, PG_CTAS) k_paged_unit(const PagedA
         float num = 0.0f, den = 0.0f;
 #pragma unroll
         for (int w = 0; w < PG_WARPS; w++) {
-            const float f = kx::ex2(red[w][h][0] - ms);
+            const float f = kx::ex2_approx(red[w][h][0] - ms);
             den += f * red[w][h][1];
             num += f * reinterpret_cast<const float*>(smem + w * (PG_STAGES * S::STAGE))[x];
         }
@@ -754,13 +747,13 @@ __device__ __forceinline__ void join_parts(const PagedArgs& A, int j, int j1, in
         float top = *m;
 #pragma unroll
         for (int u = 0; u < 8; u++) top = fmaxf(top, st[u].x);
-        const float safe = top == -INFINITY ? 0.0f : top, back = kx::ex2(*m - safe);
+        const float safe = top == -INFINITY ? 0.0f : top, back = kx::ex2_approx(*m - safe);
         *m = top;
         *den *= back;
         num->x *= back, num->y *= back, num->z *= back, num->w *= back;
 #pragma unroll
         for (int u = 0; u < 8; u++) {
-            const float f = kx::ex2(st[u].x - safe);
+            const float f = kx::ex2_approx(st[u].x - safe);
             *den += f * st[u].y;
             num->x += f * v[u].x;
             num->y += f * v[u].y;
@@ -839,7 +832,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedArgs A, int warps
                 const float safe = all == -INFINITY ? 0.0f : all;
 #pragma unroll
                 for (int z = 0; z < 8; z++) {
-                    const float f = kx::ex2(top[z] - safe);
+                    const float f = kx::ex2_approx(top[z] - safe);
                     n += f * acc[z][tid];
                     l += f * sum[z];
                 }

@@ -50,6 +50,7 @@ SIGNATURES = {
     "kx_kv_free": [_vp, _vp, _i, _vp, _vp],
     "kx_kv_compact": [_vp, _vp, _vp, _sz, _vp],
     "kx_attention_paged": [_vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _f, _vp, _i, _vp, _sz, _vp, _vp],
+    "kx_attention_window": [_vp, _i, _vp, _i, _vp, _i, _vp, _i] + [_i] * 7 + [_vp, _vp, _i, _i, _f, _vp, _sz, _vp, _vp],
     "kx_fma_relu": [_vp, _vp, _vp, _vp, _sz, _vp],
     "kx_unshard_cols": [_vp, _i, _l, _i, _vp, _i, _vp],
     "kx_rnn_step": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l, _i, _i, _i, _i, _i, _i, _i, _i, _f, _vp],
@@ -65,6 +66,7 @@ SIGNATURES = {
 SIZES = {
     "kx_kv_ws": [_vp],
     "kx_attention_paged_ws": [_vp, _i, _i],
+    "kx_attention_window_ws": [_i, _i, _i, _i, _i],
 }
 
 

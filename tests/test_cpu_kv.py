@@ -80,3 +80,25 @@ def test_paged_attention_refuses_bad_arguments(kx):
         bad = fake(kx, **kw)
         assert L.kx_attention_paged_ws(ref(bad), 4, 2) == 0 and call(c=bad) == -1, kw
     assert call(n_rows=0) == 0
+
+
+def test_window_attention_refuses_bad_arguments(kx):
+    L, p = kx.lib(), 0x60000
+    n = L.kx_attention_window_ws(2, 100, 2, 64, 48)
+    assert n > 0
+    names = ["q", "ldq", "k", "ldk", "v", "ldv", "ctx", "ldc", "B", "Rq", "S", "H", "Hkv", "dk", "dv", "q_len", "k_len", "window",
+             "sinks", "scale", "ws", "nbytes", "status", "stream"]
+    good = dict(q=p, ldq=256, k=p, ldk=128, v=p, ldv=96, ctx=p, ldc=192, B=2, Rq=5, S=100, H=4, Hkv=2, dk=64, dv=48, q_len=None,
+                k_len=None, window=0, sinks=0, scale=0.0, ws=p, nbytes=n, status=None, stream=None)
+
+    def call(**kw):
+        a = dict(good, **kw)
+        return L.kx_attention_window(*[a[x] for x in names])
+
+    for kw in [dict(q=None), dict(k=None), dict(v=None), dict(ctx=None), dict(ldq=255), dict(ldk=127), dict(ldv=95), dict(ldc=191),
+               dict(B=-1), dict(Rq=-1), dict(S=0), dict(H=3), dict(H=0), dict(Hkv=0), dict(dk=0), dict(dk=129), dict(dv=0), dict(dv=129),
+               dict(sinks=-1), dict(scale=float("nan")), dict(ws=None), dict(ws=p + 64), dict(nbytes=n - 1)]:
+        assert call(**kw) == -1, kw
+    assert call(B=0) == 0 and call(Rq=0) == 0
+    for args in [(-1, 100, 2, 64, 48), (2, 0, 2, 64, 48), (2, 100, 0, 64, 48), (2, 100, 2, 129, 48), (2, 100, 2, 64, 0)]:
+        assert L.kx_attention_window_ws(*args) == 0
