@@ -2,12 +2,14 @@
 // include/kx_kernels.h), in fp32, on the 5th-generation tensor cores. Per query row at position t and head, over the keys
 // j <= t with j > t - window or j < sinks:  ctx = sum_j p_j v_j / sum_j p_j,  p_j = exp(s_j - max s),  s_j = scale q.k_j.
 //
-// fp32 accuracy from fp16 products: an fp32 value, scaled by a power of two so that the largest of its row is in
-// [2^13, 2^14), is the sum of two fp16 parts up to 2^-22 of itself (up to 2^-39 of the row's largest where that is more),
-// and a.b = ah.bh + al.bh + ah.bl: three fp16 products where 3xTF32 (the same 11-bit parts, no scaling) would cost six
-// fp16 products' time. The scales are per query row, per key, and per 64 keys and value column, so that every
-// accumulator has one scale; they are undone in fp32 (key scales before the softmax, value scales when a tile's p.v is
-// added to the output). p in [0, 1] becomes p 2^13.
+// fp32 accuracy from fp16 products: an fp32 value, scaled by a power of two so that the largest of its query row (of its
+// 64 keys) is in [2^13, 2^14), is the sum of two fp16 parts up to 2^-22 of itself (up to 2^-39 of that largest where
+// that is more), and a.b = ah.bh + al.bh + ah.bl: three fp16 products where 3xTF32 (the same 11-bit parts, no scaling)
+// would cost six fp16 products' time. One scale per query row and one per tile of keys and of values: they are undone
+// in fp32, the scores' in the exponential's multiply-add, the values' by keeping the output in the units of the latest
+// tile (a ratio of two powers of two joins the factor by which a new maximum shrinks it). p in [0, 1] becomes p 2^13.
+// (A scale per key and per value column of a tile cost as many instructions as the rest of the softmax together:
+// 237 us where this takes XX, 4096 rows of 16 heads of 128 with a window of 2048.)
 //
 //  k_win_prep: per (sample, key-value head, tile of 64 keys) the parts of K (key-major) and V (transposed) in the
 //    128-byte-swizzled layout that the matrix instructions read, one contiguous block, so that the main kernel fetches a
@@ -20,7 +22,7 @@
 //    works on its tile, the tensor cores work on the other's. Each group keeps a softmax of its own (maximum, sum,
 //    output); the two are joined at the end.
 //    Sums: S and a tile's P.V are at most 24 accumulated steps in the tensor core, everything longer is fp32 adds.
-//  Values that the parts cannot hold (NaN, infinities, magnitudes from 2^60 on) are flagged per tile by k_win_prep; a CTA
+//  Values that the parts cannot hold (NaN, infinities, magnitudes from 2^40 on) are flagged per tile by k_win_prep; a CTA
 //  that would read a flagged tile, or has such a q, computes its rows with plain fp32 code that reads only what each
 //  row sees.
 // Every wait is bounded; a timeout records KX_STATUS_TIMEOUT in the status word and the CTA stops.
@@ -44,10 +46,10 @@ constexpr int WN_KEYS = 64;    // keys per tile
 constexpr int WN_ROWS = 128;   // rows per CTA
 constexpr int WN_GROUP = 128;  // threads of a softmax group
 constexpr int WN_THREADS = 3 * WN_GROUP;
-// registers per thread: launched with 168 (384 x 168 = 64,512); the two softmax groups take 216, the third warpgroup, of
-// which two threads fetch and issue, keeps 40: 256 x 216 + 128 x 40 = 60,416
+// registers per thread: launched with 168 (384 x 168 = 64,512); the two softmax groups take 232, the third warpgroup, of
+// which two threads fetch and issue, keeps 40: 256 x 232 + 128 x 40 = 64,512
 constexpr int WN_DMAX = 128;
-constexpr float WN_HUGE = 1152921504606846976.0f;  // 2^60
+constexpr float WN_HUGE = 1099511627776.0f;  // 2^40
 
 struct WinArgs {
     const float *q, *k, *v;
@@ -65,10 +67,18 @@ struct WinArgs {
     bool vecq, veck, vecv, vecc;
 };
 
-// a tile's block: K high planes, K low planes, V^T high, V^T low, 64 key scales, vp value scales; the flags lie behind the
-// last block
+// a tile's block: K high planes, K low planes, V^T high, V^T low; behind the last block one TileInfo per tile
+struct alignas(16) TileInfo {
+    float kscale, vscale;  // what products of its keys, its values are multiplied with
+    int plain;             // it holds values that the parts cannot
+    int pad;
+};
 __host__ __device__ inline uint32_t k_bytes(int ka) { return static_cast<uint32_t>(ka) * 2 * 8192; }
 __host__ __device__ inline uint32_t v_bytes(int vp) { return static_cast<uint32_t>(vp) * 256; }
+
+__device__ __forceinline__ TileInfo* infos(const WinArgs& A) {
+    return reinterpret_cast<TileInfo*>(A.ws + static_cast<size_t>(A.B) * A.Hkv * A.tiles * A.block);
+}
 
 __device__ __forceinline__ bool sample_lens(const WinArgs& A, int b, int* q, int* k) {
     *q = A.q_len ? A.q_len[b] : A.Rq;
@@ -101,8 +111,9 @@ __device__ __forceinline__ void parts2(float a, float b, uint32_t* hi, uint32_t*
     *lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 // the power of two that brings `top` (the largest magnitude) into [2^13, 2^14), and its inverse
-__device__ __forceinline__ float scale_up(float top, float* down) {
-    const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, -100), 126);
+// (top < 2^40; what is below 2^lowest keeps its distance to that)
+__device__ __forceinline__ float scale_up(float top, int lowest, float* down) {
+    const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, lowest), 40);
     *down = __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
     return __uint_as_float(static_cast<uint32_t>(127 + 13 - e) << 23);
 }
@@ -119,10 +130,13 @@ __device__ __forceinline__ float top4(float m, float4 x) {
 __device__ __forceinline__ bool held(float x) { return fabsf(x) < WN_HUGE; }  // false for NaN
 __device__ __forceinline__ bool held4(float4 x) { return held(x.x) && held(x.y) && held(x.z) && held(x.w); }
 
-// Bound: HBM (and L2's write rate): 8 bytes read and 8 written per element pair of K and V.
+// Bound: HBM and L2 writes, 4 bytes read and 4 written per element. A CTA per tile: both operands into shared memory,
+// their largest magnitudes, then the parts in whole 128-byte rows of the swizzled planes.
 __global__ void __launch_bounds__(256) k_win_prep(const __grid_constant__ WinArgs A) {
-    __shared__ float vs[WN_KEYS][WN_DMAX + 1];
-    __shared__ float part[8][WN_DMAX];
+    extern __shared__ float rows[];  // K, then V: 64 rows of 129
+    __shared__ float tops[2][8];
+    constexpr int P = WN_DMAX + 1;
+    float *ks = rows, *vs = rows + WN_KEYS * P;
     kx::griddep_wait();
     kx::griddep_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -135,71 +149,66 @@ __global__ void __launch_bounds__(256) k_win_prep(const __grid_constant__ WinArg
         const Tiles t = tiles_of(A, kl - ql, kl - 1);
         if (tile >= t.na && tile < t.b0) return;
     }
-    uint8_t* out = A.ws + static_cast<size_t>(blockIdx.x) * A.block;
-    float* kscale = reinterpret_cast<float*>(out + k_bytes(A.ka) + v_bytes(A.vp));
-    float* vscale = kscale + WN_KEYS;
     bool good = true;
-    // V into shared memory, and the columns' largest magnitudes
-    for (int r = warp; r < WN_KEYS; r += 8) {
-        const float* src = A.v + (static_cast<long>(b) * A.S + j0 + r) * A.ldv + h * A.dv;
-        const float4 x = r < n ? load4(src, lane * 4, A.dv, A.vecv) : make_float4(0.f, 0.f, 0.f, 0.f);
-        good = good && held4(x);
-        vs[r][lane * 4] = x.x, vs[r][lane * 4 + 1] = x.y, vs[r][lane * 4 + 2] = x.z, vs[r][lane * 4 + 3] = x.w;
+    float ktop = 0.0f, vtop = 0.0f;
+    const float* kr = A.k + (static_cast<long>(b) * A.S + j0) * A.ldk + h * A.dk;
+    const float* vr = A.v + (static_cast<long>(b) * A.S + j0) * A.ldv + h * A.dv;
+#pragma unroll 4
+    for (int r = warp; r < WN_KEYS; r += 8) {  // a warp per row; rows behind the last key are zero
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 x = r < n ? load4(kr + static_cast<long>(r) * A.ldk, lane * 4, A.dk, A.veck) : zero;
+        const float4 y = r < n ? load4(vr + static_cast<long>(r) * A.ldv, lane * 4, A.dv, A.vecv) : zero;
+        good = good && held4(x) && held4(y);
+        ktop = top4(ktop, x);
+        vtop = top4(vtop, y);
+        float *kd = ks + r * P + lane * 4, *vd = vs + r * P + lane * 4;
+        kd[0] = x.x, kd[1] = x.y, kd[2] = x.z, kd[3] = x.w;
+        vd[0] = y.x, vd[1] = y.y, vd[2] = y.z, vd[3] = y.w;
     }
-    // K: a warp per row
-    for (int r = warp; r < WN_KEYS; r += 8) {
-        const float* src = A.k + (static_cast<long>(b) * A.S + j0 + r) * A.ldk + h * A.dk;
-        const float4 x = r < n ? load4(src, lane * 4, A.dk, A.veck) : make_float4(0.f, 0.f, 0.f, 0.f);
-        good = good && held4(x);
-        float top = top4(0.0f, x);
 #pragma unroll
-        for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, d));
-        float down;
-        const float up = scale_up(top, &down);
-        if (lane == 0) kscale[r] = down;
-        uint2 hi, lo;
-        parts2(x.x * up, x.y * up, &hi.x, &lo.x);
-        parts2(x.z * up, x.w * up, &hi.y, &lo.y);
-        const int plane = lane >> 4;  // 16 lanes x 4 elements = a plane's 64
-        if (plane < A.ka) {
-            uint8_t* to = out + plane * 8192 + swz(r, (lane & 15) >> 1) + (lane & 1) * 8;
-            *reinterpret_cast<uint2*>(to) = hi;
-            *reinterpret_cast<uint2*>(to + A.ka * 8192) = lo;
-        }
+    for (int d = 16; d; d >>= 1) {
+        ktop = fmaxf(ktop, __shfl_xor_sync(FULL, ktop, d));
+        vtop = fmaxf(vtop, __shfl_xor_sync(FULL, vtop, d));
+    }
+    if (lane == 0) {
+        tops[0][warp] = ktop;
+        tops[1][warp] = vtop;
     }
     good = __syncthreads_and(good);
-    {  // column maxima: warp w over the keys 8 w .., then all
-        for (int d = lane; d < A.vp; d += 32) {
-            float top = 0.0f;
 #pragma unroll
-            for (int r = 0; r < 8; r++) top = fmaxf(top, fabsf(vs[warp * 8 + r][d]));
-            part[warp][d] = top;
-        }
-        __syncthreads();
-        for (int d = tid; d < A.vp; d += 256) {
-            float top = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 8; w++) top = fmaxf(top, part[w][d]);
-            float down;
-            part[0][d] = scale_up(top, &down);
-            vscale[d] = down;
-        }
-        __syncthreads();
+    for (int w = 0; w < 8; w++) {
+        ktop = fmaxf(ktop, tops[0][w]);
+        vtop = fmaxf(vtop, tops[1][w]);
     }
-    // V transposed: row d, 8 keys per 16-byte chunk
-    uint8_t* vout = out + k_bytes(A.ka);
-    for (int x = tid; x < A.vp * 8; x += 256) {
-        const int d = x % A.vp, c = x / A.vp;
-        const float up = part[0][d];
+    float kdown, vdown;
+    const float kup = scale_up(ktop, -100, &kdown), vup = scale_up(vtop, -40, &vdown);
+    uint8_t* out = A.ws + static_cast<size_t>(blockIdx.x) * A.block;
+    // K: chunk c of 8 head dims of key r; eight threads write a plane's row
+    for (int x = tid; x < WN_KEYS * 8 * A.ka; x += 256) {
+        const int c = x & 7, r = (x >> 3) & (WN_KEYS - 1), plane = x >> 9;
+        const float* src = ks + r * P + plane * 64 + c * 8;
         uint4 hi, lo;
         uint32_t *hw = &hi.x, *lw = &lo.x;
 #pragma unroll
-        for (int e = 0; e < 4; e++) parts2(vs[c * 8 + 2 * e][d] * up, vs[c * 8 + 2 * e + 1][d] * up, hw + e, lw + e);
-        *reinterpret_cast<uint4*>(vout + swz(d, c)) = hi;
-        *reinterpret_cast<uint4*>(vout + A.vp * 128 + swz(d, c)) = lo;
+        for (int e = 0; e < 4; e++) parts2(src[2 * e] * kup, src[2 * e + 1] * kup, hw + e, lw + e);
+        *reinterpret_cast<uint4*>(out + plane * 8192 + swz(r, c)) = hi;
+        *reinterpret_cast<uint4*>(out + (A.ka + plane) * 8192 + swz(r, c)) = lo;
     }
-    if (tid == 0) reinterpret_cast<int*>(A.ws + static_cast<size_t>(A.B) * A.Hkv * A.tiles * A.block)[blockIdx.x] = !good;
+    // V transposed: chunk c of 8 keys of head dim d
+    out += k_bytes(A.ka);
+    for (int x = tid; x < A.vp * 8; x += 256) {
+        const int c = x & 7, d = x >> 3;
+        const float* src = vs + c * 8 * P + d;
+        uint4 hi, lo;
+        uint32_t *hw = &hi.x, *lw = &lo.x;
+#pragma unroll
+        for (int e = 0; e < 4; e++) parts2(src[2 * e * P] * vup, src[(2 * e + 1) * P] * vup, hw + e, lw + e);
+        *reinterpret_cast<uint4*>(out + swz(d, c)) = hi;
+        *reinterpret_cast<uint4*>(out + A.vp * 128 + swz(d, c)) = lo;
+    }
+    if (tid == 0) infos(A)[blockIdx.x] = TileInfo{kdown, vdown, !good, 0};
 }
+constexpr int WN_PREP_SMEM = 2 * WN_KEYS * (WN_DMAX + 1) * 4;
 
 template <int D>
 struct Win {
@@ -219,8 +228,7 @@ struct WinCtl {
     uint32_t tmem;
     int abort, slow;
     float qtop[2][WN_ROWS];
-    alignas(16) float scales[2][2][WN_KEYS + WN_DMAX];  // per group, every other tile of it
-    float ml[WN_ROWS][2];
+    float ml[WN_ROWS][3];                             // the second group's maximum, sum and unit of its output
 };
 
 // The rows of a CTA in plain fp32, a warp per row: lanes over the head dims, one key after another. For inputs that the
@@ -315,16 +323,16 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     if (nq > 0) tl = tiles_of(A, off + i0, off + i0 + nq - 1);
     const int n_tiles = tl.count();
     const uint8_t* blocks = A.ws + static_cast<size_t>(bh) * A.tiles * A.block;
-    const int* flags = reinterpret_cast<const int*>(A.ws + static_cast<size_t>(A.B) * A.Hkv * A.tiles * A.block) + bh * A.tiles;
+    const TileInfo* info = infos(A) + static_cast<size_t>(bh) * A.tiles;
 
     // q's parts into tensor memory: group g takes the head dims [g D / 2, (g + 1) D / 2) of row r
     const int grp = warp >> 2, r = tid & (WN_ROWS - 1);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int my_i = r / heads, my_p = r < rows ? off + i0 + my_i : -1;
-    float cs = 0.0f;  // what a score's products are multiplied with, besides the key's scale
+    float cs = 0.0f;  // what a score's products are multiplied with, besides the tile's scale
     if (grp < 2 && nq > 0) {
         bool slow = false;
-        for (int t = tid; t < n_tiles; t += 2 * WN_GROUP) slow = slow || __ldcg(flags + tl.at(t)) != 0;
+        for (int t = tid; t < n_tiles; t += 2 * WN_GROUP) slow = slow || __ldcg(&info[tl.at(t)].plain) != 0;
         float4 f[D / 8];
         float top = 0.0f;
         const float* qr = A.q + (static_cast<long>(b) * A.Rq + i0 + my_i) * A.ldq + static_cast<long>(head0 + r % heads) * A.dk;
@@ -338,7 +346,7 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
         if (slow) ctl.slow = 1;
         kx::named_bar(1, 2 * WN_GROUP);
         float down;
-        float up = scale_up(fmaxf(ctl.qtop[0][r], ctl.qtop[1][r]), &down);
+        float up = scale_up(fmaxf(ctl.qtop[0][r], ctl.qtop[1][r]), -100, &down);
         cs = down * fabsf(A.scale2);
         if (A.scale2 < 0.0f) up = -up;
 #pragma unroll
@@ -445,99 +453,84 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
         }
         __syncwarp();
     } else {  // softmax groups
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        float o[D], m = -INFINITY, l = 0.0f;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
+        float2 o[D / 2];  // times `unit`: the row's output so far
+        float m = -INFINITY, l = 0.0f, unit = 1.0f;
 #pragma unroll
-        for (int y = 0; y < D; y++) o[y] = 0.0f;
+        for (int y = 0; y < D / 2; y++) o[y] = make_float2(0.0f, 0.0f);
         const uint32_t sm = tmem + lanes + W::GRP + grp * W::GRP_SIZE;
-        const int gt = tid & (WN_GROUP - 1), p_first = off + i0, p_last = off + i0 + nq - 1;
-        float ks_next = 0.0f, vs_next = 0.0f;
-        const auto fetch = [&](int t) {
-            if (t >= n) return;
-            const float* sc = reinterpret_cast<const float*>(blocks + static_cast<size_t>(tl.at(t)) * A.block + k_bytes(A.ka) + v_bytes(A.vp));
-            if (gt < WN_KEYS) ks_next = __ldcg(sc + gt);
-            if (gt < A.vp) vs_next = __ldcg(sc + WN_KEYS + gt);
-        };
-        bool ok = true;  // after a timeout the group still meets at its barriers
-        fetch(grp);
+        const int p_first = off + i0, p_last = off + i0 + nq - 1;
+        float2 scales = make_float2(1.0f, 1.0f);  // a tile's, fetched a tile ahead
+        if (grp < n) scales = __ldcg(reinterpret_cast<const float2*>(info + tl.at(grp)));
         for (int t = grp; t < n; t += 2) {
             const int ph = (t / 2) & 1, j0 = tl.at(t) * WN_KEYS;
-            float* scales = ctl.scales[grp][ph];
-            if (gt < WN_KEYS) scales[gt] = ks_next;
-            scales[WN_KEYS + gt] = vs_next;
-            fetch(t + 2);
-            kx::named_bar(1 + grp, WN_GROUP);
-            ok = ok && __all_sync(FULL, kx::mbar_wait(&ctl.sfull[grp], ph, &ctl.abort, A.status));
-            if (!ok) continue;
+            const float f = fmaxf(cs * scales.x, 1.17549435e-38f);  // positive: -inf stays -inf
+            const float shrink = unit * (1.0f / scales.y);           // powers of two
+            unit = scales.y;
+            if (t + 2 < n) scales = __ldcg(reinterpret_cast<const float2*>(info + tl.at(t + 2)));
+            if (!__all_sync(FULL, kx::mbar_wait(&ctl.sfull[grp], ph, &ctl.abort, A.status))) break;
             kx::tc_fence_after();
-            // every row sees every key of the tile
-            const bool whole = j0 + WN_KEYS - 1 <= p_first &&
-                               (A.window <= 0 || j0 > p_last - A.window || j0 + WN_KEYS <= A.sinks);
-            const auto sees = [&](int j) { return j <= my_p && (A.window <= 0 || j > my_p - A.window || j < A.sinks); };
-            float mx = -INFINITY;
+            float alpha;
+            {
+                // some row does not see some key of the tile
+                const bool masked = j0 + WN_KEYS - 1 > p_first || !(A.window <= 0 || j0 > p_last - A.window || j0 + WN_KEYS <= A.sinks);
+                const int from = A.window > 0 ? my_p - A.window - j0 : -1, to = my_p - j0, first = A.sinks - j0;
+                const auto load = [&](int c, uint32_t(&x)[32]) {  // products with the keys 32 c .. 32 c + 31
+                    kx::tmem_ld32(sm + c * 32, x);
+                    kx::tmem_ld32_wait(x);
+                    if (masked) {
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                uint32_t s[32];
-                kx::tmem_ld32(sm + c * 32, s);
-                kx::tmem_ld32_wait(s);
-#pragma unroll
-                for (int y = 0; y < 32; y += 4) {
-                    const float4 ks = *reinterpret_cast<const float4*>(scales + c * 32 + y);
-                    const float k4[4] = {ks.x, ks.y, ks.z, ks.w};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float v = __uint_as_float(s[y + e]) * k4[e];
-                        if (whole || sees(j0 + c * 32 + y + e)) mx = fmaxf(mx, v);
+                        for (int y = 0; y < 32; y++)
+                            if (c * 32 + y > to || (c * 32 + y <= from && c * 32 + y >= first)) x[y] = 0xFF800000u;
                     }
+                };
+                uint32_t s[2][32];  // the second time for D > 64, whose output leaves no registers to keep both
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    uint32_t(&x)[32] = s[D > 64 ? 0 : c];
+                    load(c, x);
+#pragma unroll
+                    for (int y = 0; y < 32; y++) top[y & 3] = fmaxf(top[y & 3], __uint_as_float(x[y]));
                 }
-            }
-            const float mn = mx == -INFINITY ? m : fmaxf(m, mx * cs), safe = mn == -INFINITY ? 0.0f : mn, shift = 13.0f - safe;
-            const float alpha = kx::ex2_approx(m - safe);
-            m = mn;
-            float sum = 0.0f;
+                const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                const float mn = mx == -INFINITY ? m : fmaxf(m, mx * f), safe = mn == -INFINITY ? 0.0f : mn, shift = 13.0f - safe;
+                alpha = kx::ex2_approx(m - safe);
+                m = mn;
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                uint32_t s[32], hi[16], lo[16];
-                kx::tmem_ld32(sm + c * 32, s);
-                kx::tmem_ld32_wait(s);
+                for (int c = 0; c < 2; c++) {
+                    uint32_t(&x)[32] = s[D > 64 ? 0 : c];
+                    if (D > 64) load(c, x);
+                    uint32_t hi[16], lo[16];
 #pragma unroll
-                for (int y = 0; y < 32; y += 4) {
-                    const float4 ks = *reinterpret_cast<const float4*>(scales + c * 32 + y);
-                    const float k4[4] = {ks.x, ks.y, ks.z, ks.w};
-                    float p[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        p[e] = kx::ex2_approx(fmaf(__uint_as_float(s[y + e]) * k4[e], cs, shift));
-                        if (!whole && !sees(j0 + c * 32 + y + e)) p[e] = 0.0f;
-                        sum += p[e];
+                    for (int y = 0; y < 32; y += 2) {
+                        float2 e = kx::fma2(make_float2(__uint_as_float(x[y]), __uint_as_float(x[y + 1])), make_float2(f, f), make_float2(shift, shift));
+                        e.x = kx::ex2_approx(e.x);
+                        e.y = kx::ex2_approx(e.y);
+                        sum[y / 2 & 1] = kx::add2(sum[y / 2 & 1], e);
+                        parts2(e.x, e.y, hi + y / 2, lo + y / 2);
                     }
-                    parts2(p[0], p[1], hi + y / 2, lo + y / 2);
-                    parts2(p[2], p[3], hi + y / 2 + 1, lo + y / 2 + 1);
+                    kx::tmem_st16(sm + c * 32, hi);
+                    kx::tmem_st16(sm + c * 32 + 16, lo);
                 }
-                kx::tmem_st16(sm + c * 32, hi);
-                kx::tmem_st16(sm + c * 32 + 16, lo);
+                l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
             }
-            l = l * alpha + sum;
             kx::tmem_st_wait();
             kx::tc_fence_before();
             kx::mbar_arrive(&ctl.pready[grp]);
-            ok = __all_sync(FULL, kx::mbar_wait(&ctl.ofull[grp], ph, &ctl.abort, A.status));
-            if (!ok) continue;
+            if (!__all_sync(FULL, kx::mbar_wait(&ctl.ofull[grp], ph, &ctl.abort, A.status))) break;
             kx::tc_fence_after();
+            const float2 keep = make_float2(alpha * shrink, alpha * shrink);
 #pragma unroll
             for (int c = 0; c < D; c += 32) {
                 if (c >= A.vp) continue;
-                uint32_t s[32];
-                kx::tmem_ld32(sm + WN_KEYS + c, s);
-                kx::tmem_ld32_wait(s);
+                uint32_t d[32];
+                kx::tmem_ld32(sm + WN_KEYS + c, d);
+                kx::tmem_ld32_wait(d);
 #pragma unroll
-                for (int y = 0; y < 32; y += 4) {
-                    const float4 vsc = *reinterpret_cast<const float4*>(scales + WN_KEYS + c + y);
-                    o[c + y] = fmaf(__uint_as_float(s[y]), vsc.x, o[c + y] * alpha);
-                    o[c + y + 1] = fmaf(__uint_as_float(s[y + 1]), vsc.y, o[c + y + 1] * alpha);
-                    o[c + y + 2] = fmaf(__uint_as_float(s[y + 2]), vsc.z, o[c + y + 2] * alpha);
-                    o[c + y + 3] = fmaf(__uint_as_float(s[y + 3]), vsc.w, o[c + y + 3] * alpha);
-                }
+                for (int y = 0; y < 32; y += 2)
+                    o[(c + y) / 2] = kx::fma2(o[(c + y) / 2], keep, make_float2(__uint_as_float(d[y]), __uint_as_float(d[y + 1])));
             }
             kx::tc_fence_before();
         }
@@ -549,20 +542,24 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
             if (grp == 1) {
                 ctl.ml[r][0] = m;
                 ctl.ml[r][1] = l;
+                ctl.ml[r][2] = unit;
 #pragma unroll
-                for (int y = 0; y < D; y++) other[r * (D + 1) + y] = o[y];
+                for (int y = 0; y < D / 2; y++) other[r * (D + 1) + 2 * y] = o[y].x, other[r * (D + 1) + 2 * y + 1] = o[y].y;
             }
             kx::named_bar(3, 2 * WN_GROUP);
             if (grp == 0 && r < rows && !ctl.abort) {
                 const float m1 = ctl.ml[r][0], mm = fmaxf(m, m1), safe = mm == -INFINITY ? 0.0f : mm;
-                const float f0 = kx::ex2_approx(m - safe), f1 = kx::ex2_approx(m1 - safe);
+                float f0 = kx::ex2_approx(m - safe), f1 = kx::ex2_approx(m1 - safe);
                 const float den = f0 * l + f1 * ctl.ml[r][1], inv = den == 0.0f ? 0.0f : 1.0f / den;
+                f0 *= inv, f1 *= inv;
+                const float u0 = unit, u1 = ctl.ml[r][2];
                 float* out = A.ctx + (static_cast<long>(b) * A.Rq + i0 + my_i) * A.ldc + static_cast<long>(head0 + r % heads) * A.dv;
 #pragma unroll
                 for (int y = 0; y < D; y += 4) {
                     float z[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) z[e] = (f0 * o[y + e] + f1 * other[r * (D + 1) + y + e]) * inv;
+                    for (int e = 0; e < 4; e++)
+                        z[e] = f0 * ((e & 1 ? o[(y + e) / 2].y : o[(y + e) / 2].x) * u0) + f1 * (other[r * (D + 1) + y + e] * u1);
                     if (A.vecc && y + 3 < A.dv) {
                         *reinterpret_cast<float4*>(out + y) = make_float4(z[0], z[1], z[2], z[3]);
                     } else {
@@ -595,23 +592,34 @@ bool layout_of(int B, int S, int Hkv, int dk, int dv, WinLayout* L) {
     L->tiles = (S + WN_KEYS - 1) / WN_KEYS;
     L->ka = (dk + 63) / 64;
     L->vp = (dv + 15) / 16 * 16;
-    L->block = (k_bytes(L->ka) + v_bytes(L->vp) + static_cast<uint32_t>(WN_KEYS + L->vp) * 4 + 127) / 128 * 128;
+    L->block = k_bytes(L->ka) + v_bytes(L->vp);
     const double blocks = static_cast<double>(B) * Hkv * L->tiles;
     if (blocks > 2e9) return false;
-    L->bytes = static_cast<size_t>(B) * Hkv * L->tiles * (L->block + 4) + 16;
+    L->bytes = static_cast<size_t>(B) * Hkv * L->tiles * (L->block + sizeof(TileInfo));
     return true;
+}
+
+// more dynamic shared memory than the default: asked for once per device
+int allow_smem(const void* kernel, int bytes, unsigned long long* devs_set) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return -1;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (__atomic_load_n(devs_set, __ATOMIC_ACQUIRE) & bit) return 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return -1;
+    __atomic_fetch_or(devs_set, bit, __ATOMIC_RELEASE);
+    return 0;
+}
+
+int launch_prep(const WinArgs& A, unsigned grid, cudaStream_t st) {
+    static unsigned long long devs_set = 0;
+    if (allow_smem(reinterpret_cast<const void*>(k_win_prep), WN_PREP_SMEM, &devs_set) != 0) return -1;
+    return kx::launch_pdl(k_win_prep, dim3(grid), dim3(256), WN_PREP_SMEM, st, A);
 }
 
 template <int D>
 int launch_main(const WinArgs& A, unsigned grid, cudaStream_t st) {
     static unsigned long long devs_set = 0;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return -1;
-    const unsigned long long bit = 1ull << (dev & 63);
-    if (!(__atomic_load_n(&devs_set, __ATOMIC_ACQUIRE) & bit)) {
-        if (cudaFuncSetAttribute(k_win_main<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Win<D>::SMEM) != cudaSuccess) return -1;
-        __atomic_fetch_or(&devs_set, bit, __ATOMIC_RELEASE);
-    }
+    if (allow_smem(reinterpret_cast<const void*>(k_win_main<D>), Win<D>::SMEM, &devs_set) != 0) return -1;
     return kx::launch_pdl(k_win_main<D>, dim3(grid), dim3(WN_THREADS), Win<D>::SMEM, st, A);
 }
 
@@ -653,7 +661,7 @@ int kx_attention_window(const float* q, int ldq, const float* k, int ldk, const 
     const double grid = static_cast<double>(A.qtiles) * B * Hkv * A.chunks;
     if (grid > 2e9) return -1;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (kx::launch_pdl(k_win_prep, dim3(static_cast<unsigned>(B * Hkv * L.tiles)), dim3(256), 0, st, A) != 0) return -1;
+    if (launch_prep(A, static_cast<unsigned>(B * Hkv * L.tiles), st) != 0) return -1;
     return dk <= 64 && dv <= 64 ? launch_main<64>(A, static_cast<unsigned>(grid), st) : launch_main<128>(A, static_cast<unsigned>(grid), st);
 }
 
