@@ -64,7 +64,7 @@ struct WinArgs {
     int qt, qtiles;            // queries per CTA, CTAs per sample and group
     uint32_t block;            // bytes per tile of the workspace
     float scale2;
-    bool vecq, veck, vecv, vecc;
+    bool vecq, veck, vecv;
 };
 
 // a tile's block: K high planes, K low planes, V^T high, V^T low; behind the last block one TileInfo per tile
@@ -218,7 +218,8 @@ struct Win {
     // tensor memory columns: q's parts, then per group S (P over it) and P.V
     static constexpr uint32_t QH = 0, QL = D / 2, GRP = D, GRP_SIZE = WN_KEYS + D, COLS = 512;
     static_assert(GRP + 2 * GRP_SIZE <= COLS, "tensor memory");
-    static_assert(STAGES * (KB + VB) >= WN_ROWS * (D + 1) * 4, "the second group's output fits in the stages");
+    static_assert(KB + VB >= WN_ROWS * D * 4, "q's rows fit in a stage");
+    static_assert(STAGES * (KB + VB) >= WN_ROWS * (D + 1) * 4, "the output fits in the stages");
 };
 
 struct WinCtl {
@@ -325,6 +326,24 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     const uint8_t* blocks = A.ws + static_cast<size_t>(bh) * A.tiles * A.block;
     const TileInfo* info = infos(A) + static_cast<size_t>(bh) * A.tiles;
 
+    // fetches tile t into its stage
+    const auto fetch = [&](int t) {
+        const int s = t % W::STAGES;
+        const uint8_t* src = blocks + static_cast<size_t>(tl.at(t)) * A.block;
+        uint8_t* dst = smem + s * (W::KB + W::VB);
+        if (t >= W::STAGES && !kx::mbar_wait(&ctl.kfree[s], (t / W::STAGES - 1) & 1, &ctl.abort, A.status)) return false;
+        kx::mbar_arrive_expect_tx(&ctl.kfull[s], k_bytes(A.ka));
+        kx::bulk_load(dst, src, k_bytes(A.ka), &ctl.kfull[s]);
+        // (a failed wait leaves the phase of vfull open; nothing of it is under way)
+        if (t >= W::STAGES && !kx::mbar_wait(&ctl.vfree[s], (t / W::STAGES - 1) & 1, &ctl.abort, A.status)) return false;
+        kx::mbar_arrive_expect_tx(&ctl.vfull[s], v_bytes(A.vp));
+        kx::bulk_load(dst + W::KB, src + k_bytes(A.ka), v_bytes(A.vp), &ctl.vfull[s]);
+        return true;
+    };
+    constexpr int EARLY = W::STAGES - 1;  // tiles fetched while q is prepared
+    if (warp == 8 && lane == 0)
+        for (int t = 0; t < min(n_tiles, EARLY); t++) fetch(t);
+
     // q's parts into tensor memory: group g takes the head dims [g D / 2, (g + 1) D / 2) of row r
     const int grp = warp >> 2, r = tid & (WN_ROWS - 1);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -333,15 +352,25 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     if (grp < 2 && nq > 0) {
         bool slow = false;
         for (int t = tid; t < n_tiles; t += 2 * WN_GROUP) slow = slow || __ldcg(&info[tl.at(t)].plain) != 0;
+        // rows in order into the last stage's shared memory (the fetching warp leaves it alone until the barrier below),
+        // chunk y of row x at place y ^ (x & 7); from there every thread takes its half row
+        float4* stage = reinterpret_cast<float4*>(smem + (W::STAGES - 1) * (W::KB + W::VB));
+#pragma unroll 8
+        for (int z = tid; z < WN_ROWS * (D / 4); z += 2 * WN_GROUP) {
+            const int y = z % (D / 4), x = z / (D / 4), i = x / heads;
+            const float* qr = A.q + (static_cast<long>(b) * A.Rq + i0 + i) * A.ldq + static_cast<long>(head0 + x - i * heads) * A.dk;
+            stage[x * (D / 4) + (y ^ (x & 7))] = x < rows ? load4(qr, y * 4, A.dk, A.vecq) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        kx::named_bar(1, 2 * WN_GROUP);
         float4 f[D / 8];
         float top = 0.0f;
-        const float* qr = A.q + (static_cast<long>(b) * A.Rq + i0 + my_i) * A.ldq + static_cast<long>(head0 + r % heads) * A.dk;
 #pragma unroll
         for (int y = 0; y < D / 8; y++) {
-            f[y] = r < rows ? load4(qr, grp * (D / 2) + y * 4, A.dk, A.vecq) : make_float4(0.f, 0.f, 0.f, 0.f);
+            f[y] = stage[r * (D / 4) + ((grp * (D / 8) + y) ^ (r & 7))];
             slow = slow || !held4(f[y]);
             top = top4(top, f[y]);
         }
+        kx::fence_proxy_async_smem();  // the stage is next written by bulk copies
         ctl.qtop[grp][r] = top;
         if (slow) ctl.slow = 1;
         kx::named_bar(1, 2 * WN_GROUP);
@@ -372,81 +401,82 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     if (grp == 2) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
         if (warp == 8 && lane == 0) {  // fetches the tiles
-            bool ok = true;
-            int sent = 0;
-            for (int t = 0; t < n && ok; t++, sent++) {
-                const int s = t % W::STAGES;
-                const uint8_t* src = blocks + static_cast<size_t>(tl.at(t)) * A.block;
-                uint8_t* dst = smem + s * (W::KB + W::VB);
-                if (t >= W::STAGES) ok = kx::mbar_wait(&ctl.kfree[s], (t / W::STAGES - 1) & 1, &ctl.abort, A.status);
-                if (!ok) break;
-                kx::mbar_arrive_expect_tx(&ctl.kfull[s], k_bytes(A.ka));
-                kx::bulk_load(dst, src, k_bytes(A.ka), &ctl.kfull[s]);
-                if (t >= W::STAGES) ok = kx::mbar_wait(&ctl.vfree[s], (t / W::STAGES - 1) & 1, &ctl.abort, A.status);
-                if (!ok) {  // this tile's K only
-                    const uint64_t t0 = kx::globaltimer();
-                    while (!kx::mbar_try_wait(&ctl.kfull[s], (t / W::STAGES) & 1) && kx::globaltimer() - t0 < KX_WAIT_NS) __nanosleep(256);
-                    break;
-                }
-                kx::mbar_arrive_expect_tx(&ctl.vfull[s], v_bytes(A.vp));
-                kx::bulk_load(dst + W::KB, src + k_bytes(A.ka), v_bytes(A.vp), &ctl.vfull[s]);
-            }
-            // no copy may still be under way when the CTA ends: the last ones issued complete every earlier one's phase too
-            if (!ok || ctl.abort) {
+            int sent = min(n_tiles, EARLY);
+            bool good = true;
+            for (; sent < n && good; sent++) good = fetch(sent);
+            // no copy may be under way when the CTA ends; where everything went well its last reader has seen to that
+            if (slow || !good || ctl.abort) {
+                const uint64_t t0 = kx::globaltimer();
                 for (int t = max(0, sent - W::STAGES); t < sent; t++) {
                     const int s = t % W::STAGES;
-                    const uint64_t t0 = kx::globaltimer();
                     while (!(kx::mbar_try_wait(&ctl.kfull[s], (t / W::STAGES) & 1) && kx::mbar_try_wait(&ctl.vfull[s], (t / W::STAGES) & 1)) &&
                            kx::globaltimer() - t0 < KX_WAIT_NS)
                         __nanosleep(256);
                 }
             }
-        } else if (warp == 9 && lane == 0) {  // issues the matrix instructions
-            const uint32_t base = kx::smem_u32(smem);
+        } else if (warp == 9) {  // issues the matrix instructions: the warp keeps together, one lane issues
+            const uint32_t tm = __shfl_sync(FULL, tmem, 0), base = __shfl_sync(FULL, kx::smem_u32(smem), 0);
             const uint32_t id_s = kx::idesc_f16(WN_ROWS, WN_KEYS), id_o = kx::idesc_f16(WN_ROWS, A.vp);
             const int ksteps = (A.dk + 15) / 16;
-            bool ok = true;
-            for (int t = 0; t <= n && ok; t++) {
+            const uint32_t k_lo = static_cast<uint32_t>(A.ka) * (8192 >> 4), v_lo = static_cast<uint32_t>(A.vp) * (128 >> 4);
+            bool good = true;
+            for (int t = 0; t <= n && good; t++) {
                 if (t < n) {  // S of tile t
                     const int g = t & 1, s = t % W::STAGES;
-                    ok = kx::mbar_wait(&ctl.kfull[s], (t / W::STAGES) & 1, &ctl.abort, A.status);
+                    good = kx::mbar_wait(&ctl.kfull[s], (t / W::STAGES) & 1, &ctl.abort, A.status);
                     // P of the group's tile before, which lies over S, has been used
-                    if (ok && t >= 2) ok = kx::mbar_wait(&ctl.ofull[g], ((t - 2) / 2) & 1, &ctl.abort, A.status);
-                    if (!ok) break;
-                    kx::tc_fence_after();
-                    const uint32_t d = tmem + W::GRP + g * W::GRP_SIZE, kh = base + s * (W::KB + W::VB), kl_ = kh + A.ka * 8192;
-                    for (int k = 0; k < ksteps; k++) {
-                        const uint32_t o = (k >> 2) * 8192 + (k & 3) * 32;
-                        kx::mma_f16_ts(d, tmem + W::QL + k * 8, kx::desc_sw128_kmajor(kh + o), id_s, k != 0);
-                        kx::mma_f16_ts(d, tmem + W::QH + k * 8, kx::desc_sw128_kmajor(kl_ + o), id_s, 1);
-                        kx::mma_f16_ts(d, tmem + W::QH + k * 8, kx::desc_sw128_kmajor(kh + o), id_s, 1);
+                    if (t >= 2) good = good && kx::mbar_wait(&ctl.ofull[g], ((t - 2) / 2) & 1, &ctl.abort, A.status);
+                    if (!__all_sync(FULL, good)) {
+                        good = false;
+                        break;
                     }
-                    kx::mma_commit(&ctl.sfull[g]);
-                    kx::mma_commit(&ctl.kfree[s]);
+                    kx::tc_fence_after();
+                    const uint32_t d = tm + W::GRP + g * W::GRP_SIZE;
+                    const uint64_t kh = kx::desc_sw128_kmajor(base + s * (W::KB + W::VB));
+                    if (kx::elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < D / 16; k++) {
+                            if (k >= ksteps) break;
+                            const uint64_t b = kh + (k >> 2) * (8192 >> 4) + (k & 3) * (32 >> 4);
+                            kx::mma_f16_ts(d, tm + W::QL + k * 8, b, id_s, k != 0);
+                            kx::mma_f16_ts(d, tm + W::QH + k * 8, b + k_lo, id_s, 1);
+                            kx::mma_f16_ts(d, tm + W::QH + k * 8, b, id_s, 1);
+                        }
+                        kx::mma_commit(&ctl.sfull[g]);
+                        kx::mma_commit(&ctl.kfree[s]);
+                    }
+                    __syncwarp();
                 }
                 if (t >= 1) {  // P.V of tile t - 1; P: high parts of 32 keys, their low parts, and again
                     const int u = t - 1, g = u & 1, s = u % W::STAGES;
-                    ok = kx::mbar_wait(&ctl.pready[g], (u / 2) & 1, &ctl.abort, A.status) &&
-                         kx::mbar_wait(&ctl.vfull[s], (u / W::STAGES) & 1, &ctl.abort, A.status);
-                    if (!ok) break;
-                    kx::tc_fence_after();
-                    const uint32_t p = tmem + W::GRP + g * W::GRP_SIZE, d = p + WN_KEYS;
-                    const uint32_t vh = base + s * (W::KB + W::VB) + W::KB, vl = vh + A.vp * 128;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t ph = p + (k >> 1) * 32 + (k & 1) * 8, pl = ph + 16;
-                        kx::mma_f16_ts(d, pl, kx::desc_sw128_kmajor(vh + k * 32), id_o, k != 0);
-                        kx::mma_f16_ts(d, ph, kx::desc_sw128_kmajor(vl + k * 32), id_o, 1);
-                        kx::mma_f16_ts(d, ph, kx::desc_sw128_kmajor(vh + k * 32), id_o, 1);
+                    good = kx::mbar_wait(&ctl.pready[g], (u / 2) & 1, &ctl.abort, A.status) &&
+                           kx::mbar_wait(&ctl.vfull[s], (u / W::STAGES) & 1, &ctl.abort, A.status);
+                    if (!__all_sync(FULL, good)) {
+                        good = false;
+                        break;
                     }
-                    kx::mma_commit(&ctl.ofull[g]);
-                    kx::mma_commit(&ctl.vfree[s]);
+                    kx::tc_fence_after();
+                    const uint32_t p = tm + W::GRP + g * W::GRP_SIZE, d = p + WN_KEYS;
+                    const uint64_t vh = kx::desc_sw128_kmajor(base + s * (W::KB + W::VB) + W::KB);
+                    if (kx::elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const uint32_t ph = p + (k >> 1) * 32 + (k & 1) * 8;
+                            const uint64_t b = vh + k * (32 >> 4);
+                            kx::mma_f16_ts(d, ph + 16, b, id_o, k != 0);
+                            kx::mma_f16_ts(d, ph, b + v_lo, id_o, 1);
+                            kx::mma_f16_ts(d, ph, b, id_o, 1);
+                        }
+                        kx::mma_commit(&ctl.ofull[g]);
+                        kx::mma_commit(&ctl.vfree[s]);
+                    }
+                    __syncwarp();
                 }
             }
-            if (!ok) {
+            if (!good) {
                 // matrix instructions may still be running: give them time to finish (bounded) before the tensor memory and
                 // the shared memory go away
-                kx::mma_commit(&ctl.drained);
+                if (kx::elect_one()) kx::mma_commit(&ctl.drained);
                 const uint64_t t0 = kx::globaltimer();
                 while (!kx::mbar_try_wait(&ctl.drained, 0) && kx::globaltimer() - t0 < KX_WAIT_NS) __nanosleep(256);
             }
@@ -552,22 +582,21 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                 float f0 = kx::ex2_approx(m - safe), f1 = kx::ex2_approx(m1 - safe);
                 const float den = f0 * l + f1 * ctl.ml[r][1], inv = den == 0.0f ? 0.0f : 1.0f / den;
                 f0 *= inv, f1 *= inv;
-                const float u0 = unit, u1 = ctl.ml[r][2];
-                float* out = A.ctx + (static_cast<long>(b) * A.Rq + i0 + my_i) * A.ldc + static_cast<long>(head0 + r % heads) * A.dv;
+                f0 *= unit, f1 *= ctl.ml[r][2];
 #pragma unroll
-                for (int y = 0; y < D; y += 4) {
-                    float z[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        z[e] = f0 * ((e & 1 ? o[(y + e) / 2].y : o[(y + e) / 2].x) * u0) + f1 * (other[r * (D + 1) + y + e] * u1);
-                    if (A.vecc && y + 3 < A.dv) {
-                        *reinterpret_cast<float4*>(out + y) = make_float4(z[0], z[1], z[2], z[3]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (y + e < A.dv) out[y + e] = z[e];
-                    }
+                for (int y = 0; y < D; y++) {
+                    float* z = other + r * (D + 1) + y;
+                    *z = f0 * (y & 1 ? o[y / 2].y : o[y / 2].x) + f1 * *z;
                 }
+            }
+            kx::named_bar(3, 2 * WN_GROUP);
+            for (int x = warp; x < rows && !ctl.abort; x += 8) {  // whole rows
+                const int i = x / heads;
+                float* out = A.ctx + (static_cast<long>(b) * A.Rq + i0 + i) * A.ldc + static_cast<long>(head0 + x - i * heads) * A.dv;
+                const float* z = other + x * (D + 1);
+#pragma unroll
+                for (int y = lane; y < D; y += 32)
+                    if (y < A.dv) out[y] = z[y];
             }
         } else if (!slow && grp == 0 && r < rows) {  // rows that see nothing
             float* out = A.ctx + (static_cast<long>(b) * A.Rq + i0 + my_i) * A.ldc + static_cast<long>(head0 + r % heads) * A.dv;
@@ -657,7 +686,7 @@ int kx_attention_window(const float* q, int ldq, const float* k, int ldk, const 
     A.qtiles = (Rq + A.qt - 1) / A.qt;
     A.scale2 = (scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(dk)) : scale) * 1.4426950408889634f;
     const auto vec = [](const float* p, int ld, int d) { return ((ld | d) & 3) == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-    A.vecq = vec(q, ldq, dk), A.veck = vec(k, ldk, dk), A.vecv = vec(v, ldv, dv), A.vecc = vec(ctx, ldc, dv);
+    A.vecq = vec(q, ldq, dk), A.veck = vec(k, ldk, dk), A.vecv = vec(v, ldv, dv);
     const double grid = static_cast<double>(A.qtiles) * B * Hkv * A.chunks;
     if (grid > 2e9) return -1;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
