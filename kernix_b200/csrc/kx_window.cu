@@ -106,7 +106,8 @@ __device__ __forceinline__ Tiles tiles_of(const WinArgs& A, int p0, int p1) {
 __device__ __forceinline__ void parts2(float a, float b, uint32_t* hi, uint32_t* lo) {
     const __half2 h = __floats2half2_rn(a, b);
     const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
+    const float2 rest = kx::fma2(f, make_float2(-1.0f, -1.0f), make_float2(a, b));
+    const __half2 l = __floats2half2_rn(rest.x, rest.y);
     *hi = *reinterpret_cast<const uint32_t*>(&h);
     *lo = *reinterpret_cast<const uint32_t*>(&l);
 }
@@ -355,12 +356,19 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
         // rows in order into the last stage's shared memory (the fetching warp leaves it alone until the barrier below),
         // chunk y of row x at place y ^ (x & 7); from there every thread takes its half row
         float4* stage = reinterpret_cast<float4*>(smem + (W::STAGES - 1) * (W::KB + W::VB));
-#pragma unroll 8
         for (int z = tid; z < WN_ROWS * (D / 4); z += 2 * WN_GROUP) {
             const int y = z % (D / 4), x = z / (D / 4), i = x / heads;
             const float* qr = A.q + (static_cast<long>(b) * A.Rq + i0 + i) * A.ldq + static_cast<long>(head0 + x - i * heads) * A.dk;
-            stage[x * (D / 4) + (y ^ (x & 7))] = x < rows ? load4(qr, y * 4, A.dk, A.vecq) : make_float4(0.f, 0.f, 0.f, 0.f);
+            float4* to = stage + x * (D / 4) + (y ^ (x & 7));
+            if (A.vecq) {
+                const bool in = x < rows && y * 4 < A.dk;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(kx::smem_u32(to)), "l"(in ? qr + y * 4 : A.q), "r"(in ? 16 : 0)
+                             : "memory");
+            } else {
+                *to = x < rows ? load4(qr, y * 4, A.dk, false) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         kx::named_bar(1, 2 * WN_GROUP);
         float4 f[D / 8];
         float top = 0.0f;

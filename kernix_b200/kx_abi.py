@@ -78,6 +78,7 @@ class KvCache(ctypes.Structure):
 
 
 _done = False
+_bound = {}  # entry points that were called
 
 
 def lib():
@@ -98,7 +99,10 @@ def lib():
 
 def call(name, *args):
     """Call a kx_* entry point; raises RuntimeError when it rejects the arguments or the launch fails."""
-    rc = getattr(lib(), name)(*args)
+    fn = _bound.get(name)
+    if fn is None:
+        fn = _bound[name] = getattr(lib(), name)
+    rc = fn(*args)
     if rc != 0:
         raise RuntimeError(f"{name} returned {rc}")
 
