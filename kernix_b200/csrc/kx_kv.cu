@@ -2,8 +2,8 @@
 // (fork), release (free) and moving the live pages together (compact). include/kx_kernels.h states what each does.
 //
 // All of it is bookkeeping on a few hundred KB of integers (latency) plus copies of whole pages or rows (HBM). What has
-// to be decided in order -- which free page goes to whom -- is decided by one CTA, whose warps each scan one contiguous
-// segment of the reference counts: a count per warp, one scan over the 32 counts, then every page's rank by ballot.
+// to be decided in order -- which free page goes to whom -- is decided by one CTA, whose warps each hold 1024
+// reference counts in registers: a count per warp, one scan over the 32 counts, then every page's rank by shuffles.
 // What can be done in any order (copying pages, filling table rows) is left to a second launch over the whole GPU,
 // which finds the first one's decisions in the workspace (programmatic dependent launch: its CTAs are up by then).
 // Integer atomics only where their order cannot show: counts of references, and minima.
@@ -22,8 +22,6 @@ namespace {
 
 constexpr int PLAN = 1024;  // threads of the one-CTA planners
 constexpr unsigned FULL = 0xFFFFFFFFu;
-
-inline int launch_ok() { return cudaGetLastError() == cudaSuccess ? 0 : -1; }
 
 // inclusive sum over the CTA's PLAN threads; tmp: 32 words of shared memory. *total: the sum over all.
 __device__ __forceinline__ long long block_scan(long long v, long long* tmp, long long* total) {
@@ -50,65 +48,97 @@ __device__ __forceinline__ long long block_scan(long long v, long long* tmp, lon
     return v + (warp ? tmp[warp - 1] : 0);
 }
 
-// Calls f(page, free, rank) for every page, rank = how many free pages lie below it; returns the number of free pages.
-// Every thread of the CTA takes part. Warp w scans the pages [w * seg, (w + 1) * seg), 128 at a time, four per lane.
-template <typename F>
-__device__ __forceinline__ int scan_free(const int32_t* refs, int n, int* tmp, F f) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int seg = (n + 32 * 128 - 1) / (32 * 128) * 128;
-    const long first = static_cast<long>(warp) * seg;
+// 1024 pages per warp in registers, so that a pass over up to 32768 pages waits for memory once
+constexpr int SEG = 1024, ROUND = 32 * SEG;
+struct Seg {
+    int4 r[8];  // pages first + 128 u + 4 lane ..
+    long first;
+};
+__device__ __forceinline__ int zeros(int4 r) { return (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0); }
+__device__ __forceinline__ int load_seg(const int32_t* refs, int n, long first, Seg* s) {  // returns the warp's free pages
+    const int lane = threadIdx.x & 31;
     const bool vec = (reinterpret_cast<uintptr_t>(refs) & 15) == 0;
-    const auto load = [&](long p) {
-        if (vec && p + 3 < n) return __ldcg(reinterpret_cast<const int4*>(refs + p));
+    s->first = first;
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+        const long p = first + u * 128 + lane * 4;
         int4 r = make_int4(1, 1, 1, 1);  // behind the last page: not free
-        if (p < n) r.x = __ldcg(refs + p);
-        if (p + 1 < n) r.y = __ldcg(refs + p + 1);
-        if (p + 2 < n) r.z = __ldcg(refs + p + 2);
-        if (p + 3 < n) r.w = __ldcg(refs + p + 3);
-        return r;
-    };
-    int mine = 0;
-    for (int i = 0; i < seg; i += 128) {
-        const int4 r = load(first + i + lane * 4);
-        mine += (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
+        if (vec && p + 3 < n) {
+            r = __ldcg(reinterpret_cast<const int4*>(refs + p));
+        } else {
+            if (p < n) r.x = __ldcg(refs + p);
+            if (p + 1 < n) r.y = __ldcg(refs + p + 1);
+            if (p + 2 < n) r.z = __ldcg(refs + p + 2);
+            if (p + 3 < n) r.w = __ldcg(refs + p + 3);
+        }
+        s->r[u] = r;
     }
-    mine = __reduce_add_sync(FULL, mine);
+    int c = 0;
+#pragma unroll
+    for (int u = 0; u < 8; u++) c += zeros(s->r[u]);
+    return __reduce_add_sync(FULL, c);
+}
+
+// the number of free pages; every thread of the CTA takes part, tmp: 32 words of shared memory
+__device__ __forceinline__ int count_free(const int32_t* refs, int n, int* tmp) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Seg s;
+    int mine = 0;
+    for (long p = static_cast<long>(warp) * SEG; p < n; p += ROUND) mine += load_seg(refs, n, p, &s);
     __syncthreads();
     if (lane == 0) tmp[warp] = mine;
     __syncthreads();
-    int t = tmp[lane];
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const int u = __shfl_up_sync(FULL, t, d);
-        if (lane >= d) t += u;
-    }
-    const int total = __shfl_sync(FULL, t, 31);
-    int rank = warp ? __shfl_sync(FULL, t, warp - 1) : 0;
-    for (int i = 0; i < seg; i += 128) {
-        const long p = first + i + lane * 4;
-        const int4 r = load(p);
-        const int c = (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
-        int before = c;
+    return __reduce_add_sync(FULL, tmp[lane]);
+}
+
+// Calls f(page, free, rank) for every page, rank = how many free pages lie below it; returns the number of free pages.
+// Every thread of the CTA takes part; tmp: 32 words of shared memory.
+template <typename F>
+__device__ __forceinline__ int scan_free(const int32_t* refs, int n, int* tmp, F f) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int base = 0;
+    for (long p0 = 0; p0 < n; p0 += ROUND) {
+        Seg s;
+        const int mine = load_seg(refs, n, p0 + warp * SEG, &s);
+        __syncthreads();
+        if (lane == 0) tmp[warp] = mine;
+        __syncthreads();
+        int t = tmp[lane];
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int u = __shfl_up_sync(FULL, before, d);
-            if (lane >= d) before += u;
+            const int u = __shfl_up_sync(FULL, t, d);
+            if (lane >= d) t += u;
         }
-        int at = rank + before - c;
-        rank += __shfl_sync(FULL, before, 31);
-        const int rr[4] = {r.x, r.y, r.z, r.w};
+        int rank = base + __shfl_sync(FULL, t, (warp + 31) & 31) * (warp > 0);
+        base += __shfl_sync(FULL, t, 31);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (p + e < n) f(static_cast<int>(p + e), rr[e] == 0, at);
-            at += rr[e] == 0;
+        for (int u = 0; u < 8; u++) {
+            const int c = zeros(s.r[u]);
+            int before = c;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int x = __shfl_up_sync(FULL, before, d);
+                if (lane >= d) before += x;
+            }
+            int at = rank + before - c;
+            rank += __shfl_sync(FULL, before, 31);
+            const long p = s.first + u * 128 + lane * 4;
+            const int rr[4] = {s.r[u].x, s.r[u].y, s.r[u].z, s.r[u].w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (p + e < n) f(static_cast<int>(p + e), rr[e] == 0, at);
+                at += rr[e] == 0;
+            }
         }
     }
-    return total;
+    return base;
 }
 
 // ------------------------------------------------------------------------------------------------ free
 // One CTA per listed slot. An entry is claimed by exchange, so a slot named twice is released once.
-__global__ void __launch_bounds__(256) k_kv_free(const kx_kv c, const int32_t* __restrict__ seqs, int* status) {
+__global__ void __launch_bounds__(256) k_kv_free(const kx_kv c, const int32_t* seqs, int* status) {
+    kx::griddep_wait();
+    kx::griddep_launch_dependents();
     const int s = seqs[blockIdx.x];
     if (s < 0) return;
     if (s >= c.n_seqs) {
@@ -125,64 +155,78 @@ __global__ void __launch_bounds__(256) k_kv_free(const kx_kv c, const int32_t* _
 }
 
 // ------------------------------------------------------------------------------------------------ extend
-// ws: list[n_pages] the free pages, lowest first, as far as they are asked for; upto[n_seqs] the pages asked for by the
-// slots up to this one (8 bytes each).
-__global__ void __launch_bounds__(PLAN) k_kv_extend(const kx_kv c, const int32_t* want, int32_t* granted, int32_t* list,
-                                                    long long* upto, int* status) {
+struct ExtendWs {
+    long long* upto;  // per slot: the pages asked for by the slots up to this one
+    int32_t* list;    // the free pages, lowest first, as far as they are asked for
+    int32_t* n_free;
+};
+
+__device__ __forceinline__ int pages_of(long tokens, int page) { return static_cast<int>((tokens + page - 1) >> (31 - __clz(page))); }
+
+__global__ void __launch_bounds__(PLAN) k_kv_extend_plan(const kx_kv c, const int32_t* want, const ExtendWs w) {
     __shared__ long long tmp[32];
     __shared__ int tmp_i[32];
+    kx::griddep_wait();
+    kx::griddep_launch_dependents();
     const int tid = threadIdx.x;
     const long cap = static_cast<long>(c.max_pages) * c.page;
-    const int shift = 31 - __clz(c.page);
-    const auto pages = [&](long tokens) { return static_cast<int>((tokens + c.page - 1) >> shift); };
     long long base = 0;
     for (int s0 = 0; s0 < c.n_seqs; s0 += PLAN) {
         const int s = s0 + tid;
         int need = 0;
         if (s < c.n_seqs) {
-            const int w = want[s], len = c.lens[s];
-            if (w > 0 && len >= 0 && len + static_cast<long>(w) <= cap) need = pages(len + static_cast<long>(w)) - pages(len);
+            const int more = want[s], len = c.lens[s];
+            if (more > 0 && len >= 0 && len + static_cast<long>(more) <= cap)
+                need = pages_of(len + static_cast<long>(more), c.page) - pages_of(len, c.page);
         }
         long long total;
         const long long incl = base + block_scan(need, tmp, &total);
-        if (s < c.n_seqs) upto[s] = incl;
+        if (s < c.n_seqs) w.upto[s] = incl;
         base += total;
     }
     const long long asked = base;
     const int n_free = scan_free(c.refs, c.n_pages, tmp_i, [&](int p, bool free, int rank) {
-        if (free && rank < asked) list[rank] = p;
+        if (free && rank < asked) w.list[rank] = p;
     });
-    __syncthreads();  // list and upto are written
-    const int lane = tid & 31;
-    for (int s = tid >> 5; s < c.n_seqs; s += PLAN / 32) {  // a warp per slot
-        const int w = want[s], len = c.lens[s];
-        int grant = 0;
-        if (w > 0) {
-            if (len < 0 || len > cap) {
-                if (lane == 0) kx::kv_report(status, KX_STATUS_BAD_REQUEST);
-            } else if (len + static_cast<long>(w) > cap) {
-                if (lane == 0) kx::kv_report(status, KX_STATUS_NO_PAGES);
-            } else {
-                const int have = pages(len), need = pages(len + static_cast<long>(w)) - have;
-                const long long last = upto[s];
-                if (need == 0 || last <= n_free) {
-                    grant = w;
-                    int32_t* row = c.table + static_cast<long>(s) * c.max_pages + have;
-                    for (int j = lane; j < need; j += 32) {
-                        const int p = list[last - need + j];
-                        row[j] = p;
-                        c.refs[p] = 1;
-                    }
-                } else if (lane == 0) {
-                    kx::kv_report(status, KX_STATUS_NO_PAGES);
+    if (tid == 0) *w.n_free = n_free;
+}
+
+// a warp per slot
+__global__ void __launch_bounds__(128) k_kv_extend_take(const kx_kv c, const int32_t* want, int32_t* granted, const ExtendWs w, int* status) {
+    const int lane = threadIdx.x & 31;
+    const long cap = static_cast<long>(c.max_pages) * c.page;
+    kx::griddep_wait();
+    kx::griddep_launch_dependents();
+    const int s = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (s >= c.n_seqs) return;
+    const int more = want[s], len = c.lens[s], n_free = __ldcg(w.n_free);
+    const long long last = __ldcg(w.upto + s);
+    int grant = 0;
+    if (more > 0) {
+        if (len < 0 || len > cap) {
+            if (lane == 0) kx::kv_report(status, KX_STATUS_BAD_REQUEST);
+        } else if (len + static_cast<long>(more) > cap) {
+            if (lane == 0) kx::kv_report(status, KX_STATUS_NO_PAGES);
+        } else {
+            const int have = pages_of(len, c.page), need = pages_of(len + static_cast<long>(more), c.page) - have;
+            if (need == 0 || last <= n_free) {
+                grant = more;
+                int32_t* row = c.table + static_cast<long>(s) * c.max_pages + have;
+#pragma unroll 4
+                for (int j = lane; j < need; j += 32) {
+                    const int p = __ldcg(w.list + (last - need + j));
+                    row[j] = p;
+                    c.refs[p] = 1;
                 }
+            } else if (lane == 0) {
+                kx::kv_report(status, KX_STATUS_NO_PAGES);
             }
         }
-        __syncwarp();  // every lane has read want[s] and lens[s]
-        if (lane == 0) {
-            granted[s] = grant;
-            if (grant) c.lens[s] = len + grant;
-        }
+    }
+    __syncwarp();  // every lane has read want[s] and lens[s]
+    if (lane == 0) {
+        granted[s] = grant;
+        if (grant) c.lens[s] = len + grant;
     }
 }
 
@@ -218,11 +262,13 @@ __device__ __forceinline__ uint4 kv_pack(const float* x, bool vec) {
 // CTA (s, y): rows y * rb .. of slot s; a thread converts 16 bytes of the cache at a time. HBM-bound: the fp32 rows are
 // read once (streaming loads), the narrower rows written once.
 template <int TYPE>
-__global__ void __launch_bounds__(256) k_kv_append(const kx_kv c, const float* __restrict__ k, int ldk, const float* __restrict__ v,
-                                                   int ldv, const int32_t* __restrict__ count, int rows, int rb, bool vec, long k_off,
+__global__ void __launch_bounds__(256) k_kv_append(const kx_kv c, const float* k, int ldk, const float* v,
+                                                   int ldv, const int32_t* count, int rows, int rb, bool vec, long k_off,
                                                    long v_off, int* status) {
     constexpr int E = TYPE == KX_KV_F32 ? 4 : 8;
     const int s = blockIdx.x, i0 = blockIdx.y * rb;
+    kx::griddep_wait();
+    kx::griddep_launch_dependents();
     int n = count[s];
     const int len = c.lens[s];
     if (n <= 0) return;
@@ -240,7 +286,7 @@ __global__ void __launch_bounds__(256) k_kv_append(const kx_kv c, const float* _
     for (int t = threadIdx.x; t < n * chunks; t += 256) {
         const int i = t / chunks, x = t - i * chunks;
         const int pos = len - count[s] + i0 + i;
-        const int p = __ldg(row + (pos >> shift)), slot = pos & (c.page - 1);
+        const int p = row[pos >> shift], slot = pos & (c.page - 1);
         if (p < 0 || p >= c.n_pages) {
             kx::kv_report(status, KX_STATUS_BAD_REQUEST);
             continue;
@@ -316,10 +362,10 @@ struct ForkWs {
                                               // (-1: refused) and the page copied, -1 where none is
 };
 
-__global__ void __launch_bounds__(PLAN) k_kv_fork_plan(const kx_kv c, const int32_t* __restrict__ src,
-                                                       const int32_t* __restrict__ dst, int n, const ForkWs w, int* status) {
+__global__ void __launch_bounds__(PLAN) k_kv_fork_plan(const kx_kv c, const int32_t* src, const int32_t* dst, int n, const ForkWs w, int* status) {
     __shared__ long long tmp[32];
     __shared__ int tmp_i[32];
+    kx::griddep_wait();
     kx::griddep_launch_dependents();
     const int tid = threadIdx.x;
     const long cap = static_cast<long>(c.max_pages) * c.page;
@@ -385,10 +431,10 @@ __global__ void __launch_bounds__(PLAN) k_kv_fork_plan(const kx_kv c, const int3
     }
 }
 
-__global__ void __launch_bounds__(256) k_kv_fork_move(const kx_kv c, const int32_t* __restrict__ src,
-                                                      const int32_t* __restrict__ dst, int n, const ForkWs w, const MoveArgs m,
+__global__ void __launch_bounds__(256) k_kv_fork_move(const kx_kv c, const int32_t* src, const int32_t* dst, int n, const ForkWs w, const MoveArgs m,
                                                       int* status) {
     kx::griddep_wait();
+    kx::griddep_launch_dependents();
     const int shift = 31 - __clz(c.page);
     for (int i = blockIdx.x; i < n; i += gridDim.x) {  // the children's table rows
         const int len = __ldcg(w.len + i);
@@ -425,10 +471,11 @@ struct CompactWs {
 __global__ void __launch_bounds__(PLAN) k_kv_compact_plan(const kx_kv c, const CompactWs w, int32_t* n_live_out) {
     __shared__ int tmp_i[32];
     __shared__ int n_late;
+    kx::griddep_wait();
     kx::griddep_launch_dependents();
     const int tid = threadIdx.x;
     if (tid == 0) n_late = 0;
-    const int n_live = c.n_pages - scan_free(c.refs, c.n_pages, tmp_i, [](int, bool, int) {});
+    const int n_live = c.n_pages - count_free(c.refs, c.n_pages, tmp_i);
     int mine = 0;
     scan_free(c.refs, c.n_pages, tmp_i, [&](int p, bool free, int rank) {
         if (p < n_live) {
@@ -458,6 +505,7 @@ __global__ void __launch_bounds__(PLAN) k_kv_compact_plan(const kx_kv c, const C
 __global__ void __launch_bounds__(256) k_kv_compact_move(const kx_kv c, const CompactWs w, const int32_t* n_live_p,
                                                          const MoveArgs m) {
     kx::griddep_wait();
+    kx::griddep_launch_dependents();
     const int n_late = __ldcg(w.count), n_live = __ldcg(n_live_p);
     if (n_late == 0) return;
     const long entries = static_cast<long>(c.n_seqs) * c.max_pages;
@@ -494,16 +542,18 @@ int kx_kv_free(const kx_kv* c, const int32_t* seqs, int n, int* status, void* st
     if (!kx::kv_ok(c) || n < 0) return -1;
     if (n == 0) return 0;
     if (!seqs) return -1;
-    k_kv_free<<<n, 256, 0, static_cast<cudaStream_t>(stream)>>>(*c, seqs, status);
-    return launch_ok();
+    return kx::launch_pdl(k_kv_free, dim3(n), dim3(256), 0, static_cast<cudaStream_t>(stream), *c, seqs, status);
 }
 
 int kx_kv_extend(const kx_kv* c, const int32_t* want, int32_t* granted, void* ws, size_t ws_bytes, int* status, void* stream) {
     if (!ws_ok(c, ws, ws_bytes) || !want || !granted) return -1;
-    long long* upto = static_cast<long long*>(ws);
-    int32_t* list = reinterpret_cast<int32_t*>(upto + c->n_seqs);
-    k_kv_extend<<<1, PLAN, 0, static_cast<cudaStream_t>(stream)>>>(*c, want, granted, list, upto, status);
-    return launch_ok();
+    ExtendWs w;
+    w.upto = static_cast<long long*>(ws);
+    w.n_free = reinterpret_cast<int32_t*>(w.upto + c->n_seqs);
+    w.list = w.n_free + 4;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (kx::launch_pdl(k_kv_extend_plan, dim3(1), dim3(PLAN), 0, st, *c, want, w) != 0) return -1;
+    return kx::launch_pdl(k_kv_extend_take, dim3((c->n_seqs + 3) / 4), dim3(128), 0, st, *c, want, granted, w, status);
 }
 
 int kx_kv_append(const kx_kv* c, int layer, const float* k, int ldk, const float* v, int ldv, const int32_t* count, int rows,
@@ -518,13 +568,12 @@ int kx_kv_append(const kx_kv* c, int layer, const float* k, int ldk, const float
     const long sz = kx::kv_elem_bytes(c->type);
     const long k_off = layer ? layer * c->k_layer * sz : 0, v_off = layer ? layer * c->v_layer * sz : 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (c->type == KX_KV_F32)
-        k_kv_append<KX_KV_F32><<<grid, 256, 0, st>>>(*c, k, ldk, v, ldv, count, rows, rb, vec, k_off, v_off, status);
-    else if (c->type == KX_KV_F16)
-        k_kv_append<KX_KV_F16><<<grid, 256, 0, st>>>(*c, k, ldk, v, ldv, count, rows, rb, vec, k_off, v_off, status);
-    else
-        k_kv_append<KX_KV_BF16><<<grid, 256, 0, st>>>(*c, k, ldk, v, ldv, count, rows, rb, vec, k_off, v_off, status);
-    return launch_ok();
+    const auto launch = [&](auto kernel) {
+        return kx::launch_pdl(kernel, grid, dim3(256), 0, st, *c, k, ldk, v, ldv, count, rows, rb, vec, k_off, v_off, status);
+    };
+    if (c->type == KX_KV_F32) return launch(k_kv_append<KX_KV_F32>);
+    if (c->type == KX_KV_F16) return launch(k_kv_append<KX_KV_F16>);
+    return launch(k_kv_append<KX_KV_BF16>);
 }
 
 int kx_kv_fork(const kx_kv* c, const int32_t* src, const int32_t* dst, int n, void* ws, size_t ws_bytes, int* status, void* stream) {
@@ -538,8 +587,7 @@ int kx_kv_fork(const kx_kv* c, const int32_t* src, const int32_t* dst, int n, vo
     w.from = w.len + c->n_seqs;
     w.to = w.from + c->n_seqs;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    k_kv_fork_plan<<<1, PLAN, 0, st>>>(*c, src, dst, n, w, status);
-    if (launch_ok() != 0) return -1;
+    if (kx::launch_pdl(k_kv_fork_plan, dim3(1), dim3(PLAN), 0, st, *c, src, dst, n, w, status) != 0) return -1;
     return kx::launch_pdl(k_kv_fork_move, dim3(sm_count() * 4), dim3(256), 0, st, *c, src, dst, n, w, move_args(c), status);
 }
 
@@ -552,8 +600,7 @@ int kx_kv_compact(const kx_kv* c, int32_t* n_live, void* ws, size_t ws_bytes, vo
     w.map = w.late + pages;
     w.count = w.map + pages;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    k_kv_compact_plan<<<1, PLAN, 0, st>>>(*c, w, n_live);
-    if (launch_ok() != 0) return -1;
+    if (kx::launch_pdl(k_kv_compact_plan, dim3(1), dim3(PLAN), 0, st, *c, w, n_live) != 0) return -1;
     return kx::launch_pdl(k_kv_compact_move, dim3(sm_count() * 8), dim3(256), 0, st, *c, w, static_cast<const int32_t*>(n_live), move_args(c));
 }
 
