@@ -213,24 +213,29 @@ constexpr int WN_PREP_SMEM = 2 * WN_KEYS * (WN_DMAX + 1) * 4;
 
 template <int D>
 struct Win {
-    static constexpr int STAGES = 3;
-    static constexpr int KB = D / 64 * 2 * 8192, VB = D * 256;  // bytes of a K and a V tile, at most
-    static constexpr int SMEM = STAGES * (KB + VB) + 1024;
-    // tensor memory columns: q's parts, then per group S (P over it) and P.V
-    static constexpr uint32_t QH = 0, QL = D / 2, GRP = D, GRP_SIZE = WN_KEYS + D, COLS = 512;
-    static_assert(GRP + 2 * GRP_SIZE <= COLS, "tensor memory");
-    static_assert(KB + VB >= WN_ROWS * D * 4, "q's rows fit in a stage");
-    static_assert(STAGES * (KB + VB) >= WN_ROWS * (D + 1) * 4, "the output fits in the stages");
+    static constexpr int KB = D / 64 * 2 * 8192, VB = D * 256;  // bytes of a K and a V tile, at most; three of each
+    // K and V tiles 0 and 1, K tile 2, V tile 2: q's rows as they come lie from K tile 2 on
+    static constexpr int V0 = 2 * KB, K2 = V0 + 2 * VB, V2 = K2 + KB, TOPS = V2 + VB, SMEM = TOPS + 2 * WN_ROWS * 4 + 1024;
+    // tensor memory columns: q's high and low parts, NS tiles' S (P over it), P.V of either group. With a third S a group
+    // that has stored P finds its next tile's S and may leave P.V to be added later; head dims above 64 leave no room
+    // for it (with q's low parts in shared memory they would, but those products then take half as long again).
+    static constexpr int NS = D > 64 ? 2 : 3;
+    static constexpr bool AHEAD = NS == 3;
+    static constexpr uint32_t TQH = 0, TQL = D / 2, TS = D, TO = 256, COLS = 512;
+    static_assert(TS + NS * WN_KEYS <= TO && TO + 2 * D <= COLS, "tensor memory");
+    static_assert(K2 + WN_ROWS * D * 4 <= TOPS, "q's rows fit");
+    static_assert(TOPS >= WN_ROWS * (D + 1 + 3) * 4, "the second group's output, maxima, sums and units fit in the tiles' place");
+    __device__ __forceinline__ static int k_at(int s) { return s < 2 ? s * KB : K2; }
+    __device__ __forceinline__ static int v_at(int s) { return s < 2 ? V0 + s * VB : V2; }
 };
 
 struct WinCtl {
     uint64_t kfull[3], kfree[3], vfull[3], vfree[3];  // tiles in shared memory
-    uint64_t sfull[2], pready[2], ofull[2];           // per group: S computed, P stored, P.V computed
-    uint64_t drained;                                 // after a timeout: every matrix instruction has ended
+    uint64_t sfull[3], sfree[3];                      // S computed, P over it used
+    uint64_t pready[2], ofull[2];                     // per group: P stored, P.V computed
+    uint64_t drained[2];                              // after a timeout: an issuer's matrix instructions have ended
     uint32_t tmem;
     int abort, slow;
-    float qtop[2][WN_ROWS];
-    float ml[WN_ROWS][3];                             // the second group's maximum, sum and unit of its output
 };
 
 // The rows of a CTA in plain fp32, a warp per row: lanes over the head dims, one key after another. For inputs that the
@@ -284,18 +289,22 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     const int head0 = kvh * A.G + chunk * A.per_chunk, heads = min(A.per_chunk, A.G - chunk * A.per_chunk);
 
     if (tid == 0) {
-        for (int s = 0; s < W::STAGES; s++) {
+        for (int s = 0; s < 3; s++) {
             kx::mbar_init(&ctl.kfull[s], 1);
             kx::mbar_init(&ctl.kfree[s], 1);
+            kx::mbar_init(&ctl.sfull[s], 1);
+            kx::mbar_init(&ctl.sfree[s], 1);
+        }
+        for (int s = 0; s < 3; s++) {
             kx::mbar_init(&ctl.vfull[s], 1);
             kx::mbar_init(&ctl.vfree[s], 1);
         }
         for (int g = 0; g < 2; g++) {
-            kx::mbar_init(&ctl.sfull[g], 1);
             kx::mbar_init(&ctl.pready[g], WN_GROUP);
             kx::mbar_init(&ctl.ofull[g], 1);
         }
-        kx::mbar_init(&ctl.drained, 1);
+        kx::mbar_init(&ctl.drained[0], 1);
+        kx::mbar_init(&ctl.drained[1], 1);
         ctl.abort = 0;
         ctl.slow = 0;
         kx::fence_mbar_init();
@@ -327,25 +336,28 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     const uint8_t* blocks = A.ws + static_cast<size_t>(bh) * A.tiles * A.block;
     const TileInfo* info = infos(A) + static_cast<size_t>(bh) * A.tiles;
 
-    // fetches tile t into its stage
-    const auto fetch = [&](int t) {
-        const int s = t % W::STAGES;
-        const uint8_t* src = blocks + static_cast<size_t>(tl.at(t)) * A.block;
-        uint8_t* dst = smem + s * (W::KB + W::VB);
-        if (t >= W::STAGES && !kx::mbar_wait(&ctl.kfree[s], (t / W::STAGES - 1) & 1, &ctl.abort, A.status)) return false;
+    // K (warp 8) and V (warp 10) of tile t into their places
+    const auto fetch_k = [&](int t) {
+        const int s = t % 3;
+        if (t >= 3 && !kx::mbar_wait(&ctl.kfree[s], (t / 3 - 1) & 1, &ctl.abort, A.status)) return false;
         kx::mbar_arrive_expect_tx(&ctl.kfull[s], k_bytes(A.ka));
-        kx::bulk_load(dst, src, k_bytes(A.ka), &ctl.kfull[s]);
-        // (a failed wait leaves the phase of vfull open; nothing of it is under way)
-        if (t >= W::STAGES && !kx::mbar_wait(&ctl.vfree[s], (t / W::STAGES - 1) & 1, &ctl.abort, A.status)) return false;
-        kx::mbar_arrive_expect_tx(&ctl.vfull[s], v_bytes(A.vp));
-        kx::bulk_load(dst + W::KB, src + k_bytes(A.ka), v_bytes(A.vp), &ctl.vfull[s]);
+        kx::bulk_load(smem + W::k_at(s), blocks + static_cast<size_t>(tl.at(t)) * A.block, k_bytes(A.ka), &ctl.kfull[s]);
         return true;
     };
-    constexpr int EARLY = W::STAGES - 1;  // tiles fetched while q is prepared
+    const auto fetch_v = [&](int t) {
+        const int s = t % 3;
+        if (t >= 3 && !kx::mbar_wait(&ctl.vfree[s], (t / 3 - 1) & 1, &ctl.abort, A.status)) return false;
+        kx::mbar_arrive_expect_tx(&ctl.vfull[s], v_bytes(A.vp));
+        kx::bulk_load(smem + W::v_at(s), blocks + static_cast<size_t>(tl.at(t)) * A.block + k_bytes(A.ka), v_bytes(A.vp), &ctl.vfull[s]);
+        return true;
+    };
+    constexpr int EARLY = 2;  // tiles fetched while q is prepared (K's third place is lent to q until then)
     if (warp == 8 && lane == 0)
-        for (int t = 0; t < min(n_tiles, EARLY); t++) fetch(t);
+        for (int t = 0; t < min(n_tiles, EARLY); t++) fetch_k(t);
+    if (warp == 10 && lane == 0)
+        for (int t = 0; t < min(n_tiles, EARLY); t++) fetch_v(t);
 
-    // q's parts into tensor memory: group g takes the head dims [g D / 2, (g + 1) D / 2) of row r
+    // q's parts: group g takes the head dims [g D / 2, (g + 1) D / 2) of row r
     const int grp = warp >> 2, r = tid & (WN_ROWS - 1);
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int my_i = r / heads, my_p = r < rows ? off + i0 + my_i : -1;
@@ -353,9 +365,9 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     if (grp < 2 && nq > 0) {
         bool slow = false;
         for (int t = tid; t < n_tiles; t += 2 * WN_GROUP) slow = slow || __ldcg(&info[tl.at(t)].plain) != 0;
-        // rows in order into the last stage's shared memory (the fetching warp leaves it alone until the barrier below),
-        // chunk y of row x at place y ^ (x & 7); from there every thread takes its half row
-        float4* stage = reinterpret_cast<float4*>(smem + (W::STAGES - 1) * (W::KB + W::VB));
+        // rows in order into shared memory, chunk y of row x at place y ^ (x & 7); from there every thread takes its half row
+        float4* stage = reinterpret_cast<float4*>(smem + W::K2);
+        float* tops = reinterpret_cast<float*>(smem + W::TOPS);
         for (int z = tid; z < WN_ROWS * (D / 4); z += 2 * WN_GROUP) {
             const int y = z % (D / 4), x = z / (D / 4), i = x / heads;
             const float* qr = A.q + (static_cast<long>(b) * A.Rq + i0 + i) * A.ldq + static_cast<long>(head0 + x - i * heads) * A.dk;
@@ -378,12 +390,11 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
             slow = slow || !held4(f[y]);
             top = top4(top, f[y]);
         }
-        kx::fence_proxy_async_smem();  // the stage is next written by bulk copies
-        ctl.qtop[grp][r] = top;
+        tops[grp * WN_ROWS + r] = top;
         if (slow) ctl.slow = 1;
         kx::named_bar(1, 2 * WN_GROUP);
         float down;
-        float up = scale_up(fmaxf(ctl.qtop[0][r], ctl.qtop[1][r]), -100, &down);
+        float up = scale_up(fmaxf(tops[r], tops[WN_ROWS + r]), -100, &down);
         cs = down * fabsf(A.scale2);
         if (A.scale2 < 0.0f) up = -up;
 #pragma unroll
@@ -394,10 +405,11 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                 parts2(f[y + z].x * up, f[y + z].y * up, hi + 2 * z, lo + 2 * z);
                 parts2(f[y + z].z * up, f[y + z].w * up, hi + 2 * z + 1, lo + 2 * z + 1);
             }
-            kx::tmem_st16(tmem + lanes + W::QH + grp * (D / 4) + y * 2, hi);
-            kx::tmem_st16(tmem + lanes + W::QL + grp * (D / 4) + y * 2, lo);
+            kx::tmem_st16(tmem + lanes + W::TQH + grp * (D / 4) + y * 2, hi);
+            kx::tmem_st16(tmem + lanes + W::TQL + grp * (D / 4) + y * 2, lo);
         }
         kx::tmem_st_wait();
+        kx::fence_proxy_async_smem();  // q's place is next written by bulk copies
     }
     kx::tc_fence_before();
     __syncthreads();
@@ -408,74 +420,70 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
 
     if (grp == 2) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-        if (warp == 8 && lane == 0) {  // fetches the tiles
+        if ((warp == 8 || warp == 10) && lane == 0) {  // fetch the tiles
             int sent = min(n_tiles, EARLY);
             bool good = true;
-            for (; sent < n && good; sent++) good = fetch(sent);
+            for (; sent < n; sent++) {
+                good = warp == 8 ? fetch_k(sent) : fetch_v(sent);
+                if (!good) break;
+            }
             // no copy may be under way when the CTA ends; where everything went well its last reader has seen to that
             if (slow || !good || ctl.abort) {
                 const uint64_t t0 = kx::globaltimer();
-                for (int t = max(0, sent - W::STAGES); t < sent; t++) {
-                    const int s = t % W::STAGES;
-                    while (!(kx::mbar_try_wait(&ctl.kfull[s], (t / W::STAGES) & 1) && kx::mbar_try_wait(&ctl.vfull[s], (t / W::STAGES) & 1)) &&
-                           kx::globaltimer() - t0 < KX_WAIT_NS)
-                        __nanosleep(256);
-                }
+                                uint64_t* full = warp == 8 ? ctl.kfull : ctl.vfull;
+                for (int t = max(0, sent - 3); t < sent; t++)
+                    while (!kx::mbar_try_wait(&full[t % 3], (t / 3) & 1) && kx::globaltimer() - t0 < KX_WAIT_NS) __nanosleep(256);
             }
-        } else if (warp == 9) {  // issues the matrix instructions: the warp keeps together, one lane issues
+        } else if (warp == 9 || warp == 11) {  // issue the matrix instructions: a warp keeps together, one lane issues
             const uint32_t tm = __shfl_sync(FULL, tmem, 0), base = __shfl_sync(FULL, kx::smem_u32(smem), 0);
-            const uint32_t id_s = kx::idesc_f16(WN_ROWS, WN_KEYS), id_o = kx::idesc_f16(WN_ROWS, A.vp);
-            const int ksteps = (A.dk + 15) / 16;
-            const uint32_t k_lo = static_cast<uint32_t>(A.ka) * (8192 >> 4), v_lo = static_cast<uint32_t>(A.vp) * (128 >> 4);
+            const auto wait = [&](uint64_t* bar, int parity) {
+                return __all_sync(FULL, kx::mbar_wait(bar, parity & 1, &ctl.abort, A.status)) != 0;
+            };
             bool good = true;
-            for (int t = 0; t <= n && good; t++) {
-                if (t < n) {  // S of tile t
-                    const int g = t & 1, s = t % W::STAGES;
-                    good = kx::mbar_wait(&ctl.kfull[s], (t / W::STAGES) & 1, &ctl.abort, A.status);
-                    // P of the group's tile before, which lies over S, has been used
-                    if (t >= 2) good = good && kx::mbar_wait(&ctl.ofull[g], ((t - 2) / 2) & 1, &ctl.abort, A.status);
-                    if (!__all_sync(FULL, good)) {
-                        good = false;
-                        break;
-                    }
+            if (warp == 9) {  // S of tile t, in the place of tile t - NS once P there has been used
+                const uint32_t id = kx::idesc_f16(WN_ROWS, WN_KEYS), lo = static_cast<uint32_t>(A.ka) * (8192 >> 4);
+                const int ksteps = (A.dk + 15) / 16;
+                for (int t = 0; t < n; t++) {
+                    const int s = t % 3, z = t % W::NS;
+                    good = wait(&ctl.kfull[s], t / 3) && (t < W::NS || wait(&ctl.sfree[z], t / W::NS - 1));
+                    if (!good) break;
                     kx::tc_fence_after();
-                    const uint32_t d = tm + W::GRP + g * W::GRP_SIZE;
-                    const uint64_t kh = kx::desc_sw128_kmajor(base + s * (W::KB + W::VB));
+                    const uint32_t d = tm + W::TS + z * WN_KEYS;
+                    const uint64_t kh = kx::desc_sw128_kmajor(base + W::k_at(s));
                     if (kx::elect_one()) {
 #pragma unroll
                         for (int k = 0; k < D / 16; k++) {
                             if (k >= ksteps) break;
                             const uint64_t b = kh + (k >> 2) * (8192 >> 4) + (k & 3) * (32 >> 4);
-                            kx::mma_f16_ts(d, tm + W::QL + k * 8, b, id_s, k != 0);
-                            kx::mma_f16_ts(d, tm + W::QH + k * 8, b + k_lo, id_s, 1);
-                            kx::mma_f16_ts(d, tm + W::QH + k * 8, b, id_s, 1);
+                            kx::mma_f16_ts(d, tm + W::TQL + k * 8, b, id, k != 0);
+                            kx::mma_f16_ts(d, tm + W::TQH + k * 8, b + lo, id, 1);
+                            kx::mma_f16_ts(d, tm + W::TQH + k * 8, b, id, 1);
                         }
-                        kx::mma_commit(&ctl.sfull[g]);
+                        kx::mma_commit(&ctl.sfull[z]);
                         kx::mma_commit(&ctl.kfree[s]);
                     }
                     __syncwarp();
                 }
-                if (t >= 1) {  // P.V of tile t - 1; P: high parts of 32 keys, their low parts, and again
-                    const int u = t - 1, g = u & 1, s = u % W::STAGES;
-                    good = kx::mbar_wait(&ctl.pready[g], (u / 2) & 1, &ctl.abort, A.status) &&
-                           kx::mbar_wait(&ctl.vfull[s], (u / W::STAGES) & 1, &ctl.abort, A.status);
-                    if (!__all_sync(FULL, good)) {
-                        good = false;
-                        break;
-                    }
+            } else {  // P.V of tile t; P: high parts of 32 keys, their low parts, and again
+                const uint32_t id = kx::idesc_f16(WN_ROWS, A.vp), lo = static_cast<uint32_t>(A.vp) * (128 >> 4);
+                for (int t = 0; t < n; t++) {
+                    const int g = t & 1, s = t % 3, z = t % W::NS;
+                    good = wait(&ctl.vfull[s], t / 3) && wait(&ctl.pready[g], t / 2);
+                    if (!good) break;
                     kx::tc_fence_after();
-                    const uint32_t p = tm + W::GRP + g * W::GRP_SIZE, d = p + WN_KEYS;
-                    const uint64_t vh = kx::desc_sw128_kmajor(base + s * (W::KB + W::VB) + W::KB);
+                    const uint32_t a = tm + W::TS + z * WN_KEYS, d = tm + W::TO + g * D;
+                    const uint64_t vh = kx::desc_sw128_kmajor(base + W::v_at(s));
                     if (kx::elect_one()) {
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
-                            const uint32_t ph = p + (k >> 1) * 32 + (k & 1) * 8;
+                            const uint32_t ph = a + (k >> 1) * 32 + (k & 1) * 8;
                             const uint64_t b = vh + k * (32 >> 4);
-                            kx::mma_f16_ts(d, ph + 16, b, id_o, k != 0);
-                            kx::mma_f16_ts(d, ph, b + v_lo, id_o, 1);
-                            kx::mma_f16_ts(d, ph, b, id_o, 1);
+                            kx::mma_f16_ts(d, ph + 16, b, id, k != 0);
+                            kx::mma_f16_ts(d, ph, b + lo, id, 1);
+                            kx::mma_f16_ts(d, ph, b, id, 1);
                         }
                         kx::mma_commit(&ctl.ofull[g]);
+                        kx::mma_commit(&ctl.sfree[z]);
                         kx::mma_commit(&ctl.vfree[s]);
                     }
                     __syncwarp();
@@ -484,9 +492,10 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
             if (!good) {
                 // matrix instructions may still be running: give them time to finish (bounded) before the tensor memory and
                 // the shared memory go away
-                if (kx::elect_one()) kx::mma_commit(&ctl.drained);
+                uint64_t* bar = &ctl.drained[warp == 11];
+                if (kx::elect_one()) kx::mma_commit(bar);
                 const uint64_t t0 = kx::globaltimer();
-                while (!kx::mbar_try_wait(&ctl.drained, 0) && kx::globaltimer() - t0 < KX_WAIT_NS) __nanosleep(256);
+                while (!kx::mbar_try_wait(bar, 0) && kx::globaltimer() - t0 < KX_WAIT_NS) __nanosleep(256);
             }
         }
         __syncwarp();
@@ -496,20 +505,39 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
         float m = -INFINITY, l = 0.0f, unit = 1.0f;
 #pragma unroll
         for (int y = 0; y < D / 2; y++) o[y] = make_float2(0.0f, 0.0f);
-        const uint32_t sm = tmem + lanes + W::GRP + grp * W::GRP_SIZE;
+        const uint32_t om = tmem + lanes + W::TO + grp * D;
         const int p_first = off + i0, p_last = off + i0 + nq - 1;
         float2 scales = make_float2(1.0f, 1.0f);  // a tile's, fetched a tile ahead
         if (grp < n) scales = __ldcg(reinterpret_cast<const float2*>(info + tl.at(grp)));
-        for (int t = grp; t < n; t += 2) {
-            const int ph = (t / 2) & 1, j0 = tl.at(t) * WN_KEYS;
-            const float f = fmaxf(cs * scales.x, 1.17549435e-38f);  // positive: -inf stays -inf
-            const float shrink = unit * (1.0f / scales.y);           // powers of two
-            unit = scales.y;
-            if (t + 2 < n) scales = __ldcg(reinterpret_cast<const float2*>(info + tl.at(t + 2)));
-            if (!__all_sync(FULL, kx::mbar_wait(&ctl.sfull[grp], ph, &ctl.abort, A.status))) break;
+        float keep = 1.0f, keep_next = 1.0f;
+        const auto join = [&](int t) {  // P.V of tile t joins the output
+            if (!__all_sync(FULL, kx::mbar_wait(&ctl.ofull[grp], (t / 2) & 1, &ctl.abort, A.status))) return false;
             kx::tc_fence_after();
-            float alpha;
-            {
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                if (c >= A.vp) continue;
+                uint32_t d[32];
+                kx::tmem_ld32(om + c, d);
+                kx::tmem_ld32_wait(d);
+#pragma unroll
+                for (int y = 0; y < 32; y += 2)
+                    o[(c + y) / 2] = kx::fma2(o[(c + y) / 2], make_float2(keep, keep),
+                                              make_float2(__uint_as_float(d[y]), __uint_as_float(d[y + 1])));
+            }
+            kx::tc_fence_before();
+            return true;
+        };
+        for (int t = grp; grp < n; t += 2) {
+            if (t < n) {  // P of tile t
+                const uint32_t sm = tmem + lanes + W::TS + (t % W::NS) * WN_KEYS;
+                const int j0 = tl.at(t) * WN_KEYS;
+                const float f = fmaxf(cs * scales.x, 1.17549435e-38f);  // positive: -inf stays -inf
+                const float shrink = unit * (1.0f / scales.y);           // powers of two
+                unit = scales.y;
+                if (t + 2 < n) scales = __ldcg(reinterpret_cast<const float2*>(info + tl.at(t + 2)));
+                if (!__all_sync(FULL, kx::mbar_wait(&ctl.sfull[t % W::NS], (t / W::NS) & 1, &ctl.abort, A.status))) break;
+                kx::tc_fence_after();
+                float alpha;
                 // some row does not see some key of the tile
                 const bool masked = j0 + WN_KEYS - 1 > p_first || !(A.window <= 0 || j0 > p_last - A.window || j0 + WN_KEYS <= A.sinks);
                 const int from = A.window > 0 ? my_p - A.window - j0 : -1, to = my_p - j0, first = A.sinks - j0;
@@ -553,44 +581,36 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                     kx::tmem_st16(sm + c * 32 + 16, lo);
                 }
                 l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+                keep_next = alpha * shrink;
             }
+            if (W::AHEAD && t >= 2 && !join(t - 2)) break;
+            if (t >= n) break;
+            keep = keep_next;
             kx::tmem_st_wait();
             kx::tc_fence_before();
             kx::mbar_arrive(&ctl.pready[grp]);
-            if (!__all_sync(FULL, kx::mbar_wait(&ctl.ofull[grp], ph, &ctl.abort, A.status))) break;
-            kx::tc_fence_after();
-            const float2 keep = make_float2(alpha * shrink, alpha * shrink);
-#pragma unroll
-            for (int c = 0; c < D; c += 32) {
-                if (c >= A.vp) continue;
-                uint32_t d[32];
-                kx::tmem_ld32(sm + WN_KEYS + c, d);
-                kx::tmem_ld32_wait(d);
-#pragma unroll
-                for (int y = 0; y < 32; y += 2)
-                    o[(c + y) / 2] = kx::fma2(o[(c + y) / 2], keep, make_float2(__uint_as_float(d[y]), __uint_as_float(d[y + 1])));
-            }
-            kx::tc_fence_before();
+            if (!W::AHEAD && !join(t)) break;
         }
         // the second group's rows through shared memory (the stages: every matrix instruction that read them is done once
         // both groups have seen their last P.V), then the first group writes
         if (n > 0) {
             float* other = reinterpret_cast<float*>(smem);
+            float* ml = other + WN_ROWS * (D + 1) + r * 3;  // the second group's maximum, sum and unit
             kx::named_bar(3, 2 * WN_GROUP);
             if (grp == 1) {
-                ctl.ml[r][0] = m;
-                ctl.ml[r][1] = l;
-                ctl.ml[r][2] = unit;
+                ml[0] = m;
+                ml[1] = l;
+                ml[2] = unit;
 #pragma unroll
                 for (int y = 0; y < D / 2; y++) other[r * (D + 1) + 2 * y] = o[y].x, other[r * (D + 1) + 2 * y + 1] = o[y].y;
             }
             kx::named_bar(3, 2 * WN_GROUP);
             if (grp == 0 && r < rows && !ctl.abort) {
-                const float m1 = ctl.ml[r][0], mm = fmaxf(m, m1), safe = mm == -INFINITY ? 0.0f : mm;
+                const float m1 = ml[0], mm = fmaxf(m, m1), safe = mm == -INFINITY ? 0.0f : mm;
                 float f0 = kx::ex2_approx(m - safe), f1 = kx::ex2_approx(m1 - safe);
-                const float den = f0 * l + f1 * ctl.ml[r][1], inv = den == 0.0f ? 0.0f : 1.0f / den;
+                const float den = f0 * l + f1 * ml[1], inv = den == 0.0f ? 0.0f : 1.0f / den;
                 f0 *= inv, f1 *= inv;
-                f0 *= unit, f1 *= ctl.ml[r][2];
+                f0 *= unit, f1 *= ml[2];
 #pragma unroll
                 for (int y = 0; y < D; y++) {
                     float* z = other + r * (D + 1) + y;
