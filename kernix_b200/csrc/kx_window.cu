@@ -9,19 +9,24 @@
 // in fp32, the scores' in the exponential's multiply-add, the values' by keeping the output in the units of the latest
 // tile (a ratio of two powers of two joins the factor by which a new maximum shrinks it). p in [0, 1] becomes p 2^13.
 // (A scale per key and per value column of a tile cost as many instructions as the rest of the softmax together:
-// 237 us where this takes XX, 4096 rows of 16 heads of 128 with a window of 2048.)
+// 237 us against 224 for 4096 rows of 16 heads of 128 with a window of 2048, before the steps that made it 179.)
 //
 //  k_win_prep: per (sample, key-value head, tile of 64 keys) the parts of K (key-major) and V (transposed) in the
 //    128-byte-swizzled layout that the matrix instructions read, one contiguous block, so that the main kernel fetches a
 //    tile by two bulk copies and every CTA that reads it is spared the conversion. Tiles that no query sees are skipped.
 //  k_win_main: one CTA per (sample, key-value head, 128 rows); a row is one query of one of the G heads that share the
-//    keys (128 / G queries), so that few queries still fill the tile and a window's edges are short. Roles: a warp that
-//    fetches tiles (ring of stages), a thread that issues the matrix instructions, and two groups of 128 threads, each
-//    with every second tile: thread = row, S out of tensor memory, maximum, exponentials, P's parts back into tensor
-//    memory over S (the A operand of P.V), then the tile's P.V added to the row's output in registers. While one group
-//    works on its tile, the tensor cores work on the other's. Each group keeps a softmax of its own (maximum, sum,
-//    output); the two are joined at the end.
+//    keys (128 / G queries), so that few queries still fill the tile and a window's edges are short. Two warps fetch K and
+//    V tiles (three places each), two issue S = Q.K^T and P.V, and two groups of 128 threads take every second tile:
+//    thread = row, S out of tensor memory, maximum, exponentials, P's parts back into tensor memory over S (the A operand
+//    of P.V), the tile's P.V added to the row's output in registers. While one group works on its tile the tensor cores
+//    work on the other's. Each group keeps a softmax of its own (maximum, sum, output); the two are joined at the end.
 //    Sums: S and a tile's P.V are at most 24 accumulated steps in the tensor core, everything longer is fp32 adds.
+//    Bound: the chain S -> softmax -> P.V of a group and, close to it, the tensor cores (for heads of 128 a tile's
+//    products are 1536 cycles of tensor work; measured 2240 per tile, in which each group's softmax is 1500 of its 4480)
+//    plus a CTA's beginning and end, one fifth of its time. 16384 rows of 16 heads of 128 over 4 key-value heads with a
+//    window of 2048: 771 us, 335 TFLOP/s of fp32 products; three fp16 products at the measured matrix rate are 461 us.
+//    One issuing thread for both products stood in its own way with heads of 64, whose products are short (a matrix
+//    instruction takes about 45 cycles to issue): 124 us against 111.
 //  Values that the parts cannot hold (NaN, infinities, magnitudes from 2^40 on) are flagged per tile by k_win_prep; a CTA
 //  that would read a flagged tile, or has such a q, computes its rows with plain fp32 code that reads only what each
 //  row sees.
@@ -704,7 +709,8 @@ int kx_attention_window(const float* q, int ldq, const float* k, int ldk, const 
     A.ws = static_cast<uint8_t*>(ws);
     A.status = status;
     A.ldq = ldq, A.ldk = ldk, A.ldv = ldv, A.ldc = ldc, A.B = B, A.Rq = Rq, A.S = S, A.H = H, A.Hkv = Hkv, A.dk = dk, A.dv = dv;
-    A.window = window, A.sinks = sinks;
+    // every position is below S: a window of S sees all there is (and no sum with it passes 32 bits)
+    A.window = window >= S ? 0 : window, A.sinks = std::min(sinks, S);
     A.G = H / Hkv;
     A.chunks = (A.G + WN_ROWS - 1) / WN_ROWS;
     A.per_chunk = (A.G + A.chunks - 1) / A.chunks;

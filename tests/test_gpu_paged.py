@@ -138,6 +138,12 @@ def test_long_and_many_rows(kx, dtype, lens, window, sinks):
     assert torch.equal(first, again)
 
 
+@pytest.mark.parametrize("window,sinks", [(2**31 - 1, 2**31 - 1), (2**31 - 1, 0), (3, 2**31 - 1)])
+def test_largest_windows(kx, window, sinks):
+    c = Case([700, 1, 0, 16], 2, 2, 64, 64, 16, "bf16", window, sinks)
+    c.check(c.run(kx))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 def test_infinities_in_masked_places_and_layers(kx, dtype):
     c = Case([100, 31, 64], 2, 2, 64, 64, 16, dtype, window=10, sinks=2, layers=3, layer=2, fill=float("inf"))

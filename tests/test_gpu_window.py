@@ -227,6 +227,15 @@ def test_bad_lengths(kx):
         assert bool(good.isfinite().all())
 
 
+@pytest.mark.parametrize("window,sinks", [(2**31 - 1, 2**31 - 1), (2**31 - 1, 0), (70, 2**31 - 1), (69, 2**31 - 1)])
+def test_largest_windows(kx, window, sinks):
+    """the largest numbers, with queries before the first key"""
+    c = Case(2, 90, 70, 3, 1, 32, 32, window, sinks, q_len=[90, 70], k_len=[70, 70])
+    ctx = c.run(kx)
+    c.check(ctx)
+    assert not ctx[:20].any()
+
+
 def test_as_kx_attention(kx):
     """without a window the causal case of the library's attention"""
     c = Case(3, 128, 128, 8, 8, 64, 64)
