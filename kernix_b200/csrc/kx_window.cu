@@ -229,7 +229,7 @@ struct Win {
     static constexpr uint32_t TQH = 0, TQL = D / 2, TS = D, TO = 256, COLS = 512;
     static_assert(TS + NS * WN_KEYS <= TO && TO + 2 * D <= COLS, "tensor memory");
     static_assert(K2 + WN_ROWS * D * 4 <= TOPS, "q's rows fit");
-    static_assert(TOPS >= WN_ROWS * (D + 1 + 3) * 4, "the second group's output, maxima, sums and units fit in the tiles' place");
+    static_assert(TOPS >= WN_ROWS * (D + 2 + 6) * 4, "the groups' halves, maxima, sums and units fit in the tiles' place");
     __device__ __forceinline__ static int k_at(int s) { return s < 2 ? s * KB : K2; }
     __device__ __forceinline__ static int v_at(int s) { return s < 2 ? V0 + s * VB : V2; }
 };
@@ -369,13 +369,15 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     float cs = 0.0f;  // what a score's products are multiplied with, besides the tile's scale
     if (grp < 2 && nq > 0) {
         bool slow = false;
-        for (int t = tid; t < n_tiles; t += 2 * WN_GROUP) slow = slow || __ldcg(&info[tl.at(t)].plain) != 0;
         // rows in order into shared memory, chunk y of row x at place y ^ (x & 7); from there every thread takes its half row
         float4* stage = reinterpret_cast<float4*>(smem + W::K2);
         float* tops = reinterpret_cast<float*>(smem + W::TOPS);
-        for (int z = tid; z < WN_ROWS * (D / 4); z += 2 * WN_GROUP) {
-            const int y = z % (D / 4), x = z / (D / 4), i = x / heads;
-            const float* qr = A.q + (static_cast<long>(b) * A.Rq + i0 + i) * A.ldq + static_cast<long>(head0 + x - i * heads) * A.dk;
+        constexpr int STEP = 2 * WN_GROUP / (D / 4);  // rows at a time
+        const int y = tid % (D / 4), di = STEP / heads, dh = STEP - di * heads;
+        int i = tid / (D / 4) / heads, h = tid / (D / 4) - i * heads;
+#pragma unroll 4
+        for (int x = tid / (D / 4); x < WN_ROWS; x += STEP) {
+            const float* qr = A.q + (static_cast<long>(b) * A.Rq + i0 + i) * A.ldq + static_cast<long>(head0 + h) * A.dk;
             float4* to = stage + x * (D / 4) + (y ^ (x & 7));
             if (A.vecq) {
                 const bool in = x < rows && y * 4 < A.dk;
@@ -384,7 +386,10 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
             } else {
                 *to = x < rows ? load4(qr, y * 4, A.dk, false) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
+            i += di, h += dh;
+            if (h >= heads) h -= heads, i++;
         }
+        for (int t = tid; t < n_tiles; t += 2 * WN_GROUP) slow = slow || __ldcg(&info[tl.at(t)].plain) != 0;
         asm volatile("cp.async.wait_all;" ::: "memory");
         kx::named_bar(1, 2 * WN_GROUP);
         float4 f[D / 8];
@@ -596,40 +601,46 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
             kx::mbar_arrive(&ctl.pready[grp]);
             if (!W::AHEAD && !join(t)) break;
         }
-        // the second group's rows through shared memory (the stages: every matrix instruction that read them is done once
-        // both groups have seen their last P.V), then the first group writes
+        // the groups' rows through shared memory (the tiles' place: every matrix instruction that read them is done once both
+        // groups have seen their last P.V): each joins one half of the columns, then whole rows are written
         if (n > 0) {
-            float* other = reinterpret_cast<float*>(smem);
-            float* ml = other + WN_ROWS * (D + 1) + r * 3;  // the second group's maximum, sum and unit
+            constexpr int P = D / 2 + 1;
+            float* half = reinterpret_cast<float*>(smem);  // [group that joins it][row][column]
+            float* ml = half + 2 * WN_ROWS * P;            // [group][row]: maximum, sum and unit
             kx::named_bar(3, 2 * WN_GROUP);
-            if (grp == 1) {
-                ml[0] = m;
-                ml[1] = l;
-                ml[2] = unit;
+            float* mine = ml + (grp * WN_ROWS + r) * 3;
+            mine[0] = m, mine[1] = l, mine[2] = unit;
+            float* send = half + ((grp ^ 1) * WN_ROWS + r) * P;
 #pragma unroll
-                for (int y = 0; y < D / 2; y++) other[r * (D + 1) + 2 * y] = o[y].x, other[r * (D + 1) + 2 * y + 1] = o[y].y;
+            for (int x = 0; x < D / 4; x++) {
+                const float2 v = grp == 0 ? o[D / 4 + x] : o[x];
+                send[2 * x] = v.x, send[2 * x + 1] = v.y;
             }
             kx::named_bar(3, 2 * WN_GROUP);
-            if (grp == 0 && r < rows && !ctl.abort) {
-                const float m1 = ml[0], mm = fmaxf(m, m1), safe = mm == -INFINITY ? 0.0f : mm;
-                float f0 = kx::ex2_approx(m - safe), f1 = kx::ex2_approx(m1 - safe);
-                const float den = f0 * l + f1 * ml[1], inv = den == 0.0f ? 0.0f : 1.0f / den;
-                f0 *= inv, f1 *= inv;
-                f0 *= unit, f1 *= ml[2];
+            {
+                const float* his = ml + ((grp ^ 1) * WN_ROWS + r) * 3;
+                const float mm = fmaxf(m, his[0]), safe = mm == -INFINITY ? 0.0f : mm;
+                float f0 = kx::ex2_approx(m - safe), f1 = kx::ex2_approx(his[0] - safe);
+                const float den = f0 * l + f1 * his[1], inv = den == 0.0f ? 0.0f : 1.0f / den;
+                f0 *= inv * unit, f1 *= inv * his[2];
+                float* z = half + (grp * WN_ROWS + r) * P;
 #pragma unroll
-                for (int y = 0; y < D; y++) {
-                    float* z = other + r * (D + 1) + y;
-                    *z = f0 * (y & 1 ? o[y / 2].y : o[y / 2].x) + f1 * *z;
+                for (int x = 0; x < D / 4; x++) {
+                    const float2 v = grp == 0 ? o[x] : o[D / 4 + x];
+                    z[2 * x] = f0 * v.x + f1 * z[2 * x];
+                    z[2 * x + 1] = f0 * v.y + f1 * z[2 * x + 1];
                 }
             }
             kx::named_bar(3, 2 * WN_GROUP);
-            for (int x = warp; x < rows && !ctl.abort; x += 8) {  // whole rows
-                const int i = x / heads;
-                float* out = A.ctx + (static_cast<long>(b) * A.Rq + i0 + i) * A.ldc + static_cast<long>(head0 + x - i * heads) * A.dv;
-                const float* z = other + x * (D + 1);
+            const int di = 8 / heads, dh = 8 - di * heads;
+            int i = warp / heads, h = warp - i * heads;
+            for (int x = warp; x < rows && !ctl.abort; x += 8) {
+                float* out = A.ctx + (static_cast<long>(b) * A.Rq + i0 + i) * A.ldc + static_cast<long>(head0 + h) * A.dv;
 #pragma unroll
-                for (int y = lane; y < D; y += 32)
-                    if (y < A.dv) out[y] = z[y];
+                for (int c = 0; c < D; c += 32)
+                    if (c + lane < A.dv) out[c + lane] = half[(c < D / 2 ? 0 : WN_ROWS * P) + x * P + c % (D / 2) + lane];
+                i += di, h += dh;
+                if (h >= heads) h -= heads, i++;
             }
         } else if (!slow && grp == 0 && r < rows) {  // rows that see nothing
             float* out = A.ctx + (static_cast<long>(b) * A.Rq + i0 + my_i) * A.ldc + static_cast<long>(head0 + r % heads) * A.dv;
