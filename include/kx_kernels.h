@@ -320,7 +320,7 @@ KERNIX_API int kx_kv_compact(const kx_kv* c, int32_t* n_live, void* ws, size_t w
  * when window <= 0, or j > lens - 1 - window, or j < sinks. ctx + i * ldc receives H * dv floats. scale 0 means
  * 1/sqrt(dk). A row with seqs[i] < 0 is left as it was, one whose slot holds no tokens becomes 0, and one whose slot,
  * length or (visible) pages are out of range becomes NaN and is reported. Keys and values that are not seen do not affect
- * results, whatever they hold; those that are have to be finite (a head that sees an infinite key becomes NaN, a column
+ * results, whatever they hold; those that are have to be finite and, in an fp32 cache, below 2^127 (a head that sees an infinite key becomes NaN, a column
  * with an infinite value NaN). H a multiple of heads, dk, dv <= 128. q and ctx
  * must not overlap each other or the cache. ws: kx_attention_paged_ws bytes of device workspace (0: the arguments are
  * invalid), to be shared under kx_kv_ws's rules. Results do not depend on timing: the same call on the same contents

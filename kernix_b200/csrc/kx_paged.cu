@@ -10,7 +10,8 @@
 //     key-value head on). The cache's elements enter exactly as they are stored; the fp32 side (q, then p) is split into
 //     parts of the cache's type, whose products land in rows 0-7 (part 1) and 8-15 (part 2) of the same tile:
 //       f16:  2 parts of 11 bits, q scaled by a power of two per head to use f16's range, p in [0, 2^13];
-//       bf16: 3 parts of 8 bits, the third as a second product;
+//       bf16: 3 parts of 8 bits, the third as a second product, or in rows 4-7 where the tile has at most four heads
+//             (half the matrix instructions: 32 ragged rows 20.2 -> 18.2 us of GPU time);
 //       f32:  tf32 halves, q.k = qh.kh + ql.kh + qh.kl (and p.v likewise), 11 + 11 bits.
 //     That keeps fp32's accuracy (parts lost: below 2^-22 of the operand). A step's p.v is added to the output in
 //     fp32 registers by CUDA-core adds, not carried through the tensor core's truncating accumulation.
@@ -150,14 +151,16 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, float* ra, float* rb
     }
     return w;
 }
-// v = hi + rest with 11 bits in hi (cut off, two instructions; the tensor core cuts rest to 11 bits: 2^-21 of v is lost)
+// v = hi + rest with 11 bits in hi, to nearest: rest is at most 2^-12 of v and the tensor core cuts it to 11 bits, 2^-22
+// of v at most (cutting hi off as well saves an instruction and costs four times the error). |v| < 2^127.
 __device__ __forceinline__ uint32_t tf32_of(float v, float* rest) {
-    const uint32_t hi = __float_as_uint(v) & 0xFFFFE000u;
+    const uint32_t hi = (__float_as_uint(v) + 0x1000u) & 0xFFFFE000u;
     *rest = v - __uint_as_float(hi);
     return hi;
 }
 
-template <int TYPE, int D>
+// FEW: a bf16 cache and at most four heads per tile, whose rows 4-7 then take the third parts
+template <int TYPE, int D, bool FEW = false>
 struct Shape {
     static constexpr int EPC = TYPE == KX_KV_F32 ? 4 : 8;   // elements per 16-byte chunk
     static constexpr int KT = TYPE == KX_KV_F32 ? 1 : 2;    // tiles of 8 keys per step
@@ -173,6 +176,7 @@ struct Shape {
     static constexpr int STAGE = 2 * TILE;                  // bytes per warp and stage
     static constexpr int QW = D / 4;                        // q elements per lane
     static constexpr int PARTS = TYPE == KX_KV_BF16 ? 3 : 2;
+    static constexpr int KEPT = FEW ? 2 : PARTS;                // parts in a lane's registers
     static constexpr int QP = TYPE == KX_KV_F32 ? QW : QW / 2;  // 32-bit words per part
     static constexpr int SMEM = PG_WARPS * PG_STAGES * STAGE;
     static_assert(PG_STAGES * STAGE >= PG_HEADS * DV * 4, "a warp's ring holds its partial output");
@@ -287,10 +291,10 @@ struct Feed {
 // (g, t) holds head g; after the last step its sum is that of its own columns only.
 // Column n of a tile's scores is the key in row (n >> 1) + 4 (n & 1) of its eight (a lane's columns 2 t and 2 t + 1:
 // rows t and t + 4), and lane g reads its values in chunk (g >> 1) + 4 (g & 1) of eight: the orders without conflicts.
-template <int TYPE, int D>
+template <int TYPE, int D, bool FEW>
 struct Tile {
-    using S = Shape<TYPE, D>;
-    uint32_t qp[S::PARTS][S::QP];
+    using S = Shape<TYPE, D, FEW>;
+    uint32_t qp[S::KEPT][S::QP];
     float2 o[S::NO / 2];  // o[EPC c + e]: elements e of chunks 8 c + t and 8 c + t + 4
     float m, l, qscale, off;
 
@@ -299,7 +303,7 @@ struct Tile {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         const int kvh = c.unit / A.chunks, head0 = kvh * A.G + (c.unit - kvh * A.chunks) * A.per_chunk;
         const int heads = min(A.per_chunk, (kvh + 1) * A.G - head0);
-        const float* qr = A.q + static_cast<long>(c.row) * A.ldq + static_cast<long>(head0 + min(g, heads - 1)) * A.c.dk;
+        const float* qr = A.q + static_cast<long>(c.row) * A.ldq + static_cast<long>(head0 + min(FEW ? g & 3 : g, heads - 1)) * A.c.dk;
         float x[S::QW];
 #pragma unroll
         for (int k = 0; k < S::KCH; k++)
@@ -340,8 +344,12 @@ struct Tile {
 #pragma unroll
             for (int k = 0; k < S::QP; k++) {
                 float a = x[2 * k], b = x[2 * k + 1];
+                uint32_t w[S::PARTS];
 #pragma unroll
-                for (int p = 0; p < S::PARTS; p++) qp[p][k] = pack2<TYPE>(a, b, &a, &b);
+                for (int p = 0; p < S::PARTS; p++) w[p] = pack2<TYPE>(a, b, &a, &b);
+#pragma unroll
+                for (int p = 0; p < S::KEPT; p++) qp[p][k] = w[p];
+                if (FEW && g >= 4) qp[0][k] = w[S::PARTS - 1], qp[1][k] = 0;
             }
         }
 #pragma unroll
@@ -381,13 +389,19 @@ struct Tile {
                 } else {
                     mma_bf16(d, qp[0][x], qp[1][x], qp[0][x + 1], qp[1][x + 1], kv.x, kv.y);
                     mma_bf16(d, qp[0][x + 2], qp[1][x + 2], qp[0][x + 3], qp[1][x + 3], kv.z, kv.w);
-                    mma_bf16(f, qp[2][x], 0, qp[2][x + 1], 0, kv.x, kv.y);
-                    mma_bf16(f, qp[2][x + 2], 0, qp[2][x + 3], 0, kv.z, kv.w);
+                    if constexpr (!FEW) {
+                        mma_bf16(f, qp[2][x], 0, qp[2][x + 1], 0, kv.x, kv.y);
+                        mma_bf16(f, qp[2][x + 2], 0, qp[2][x + 3], 0, kv.z, kv.w);
+                    }
                 }
             }
 #pragma unroll
             for (int e = 0; e < 2; e++)
                 s[2 * u + e] = ((dd[0][e] + dd[1][e]) + ((dd[0][e + 2] + dd[1][e + 2]) + (dd[2][e] + dd[3][e]))) * qscale;
+            if (FEW) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) s[2 * u + e] += __shfl_xor_sync(FULL, s[2 * u + e], 16);
+            }
         }
         if (!c.whole()) {
             const int j = c.first_key() + t;
@@ -444,6 +458,7 @@ struct Tile {
                     pa[x] = pack2<TYPE>(a, b, &a, &b);
                     pb[x] = pack2<TYPE>(cc, d, &cc, &d);
                 }
+                if (FEW && g >= 4) pa[0] = pa[S::PARTS - 1], pb[0] = pb[S::PARTS - 1], pa[1] = pb[1] = 0;
             }
 #pragma unroll
             for (int k = 0; k < S::VCH; k++) {
@@ -461,7 +476,7 @@ struct Tile {
                     if constexpr (TYPE == KX_KV_F16) {
                         mma_f16(d, pa[0], pa[1], pb[0], pb[1], b0, b1);
                     } else {
-                        mma_bf16(d, pa[2], 0, pb[2], 0, b0, b1);
+                        if constexpr (!FEW) mma_bf16(d, pa[2], 0, pb[2], 0, b0, b1);
                         mma_bf16(d, pa[0], pa[1], pb[0], pb[1], b0, b1);
                     }
                     o[k * 8 + e] = add2(o[k * 8 + e], add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])));
@@ -474,6 +489,13 @@ struct Tile {
         l += __shfl_xor_sync(FULL, l, 1);
         l += __shfl_xor_sync(FULL, l, 2);
         if (bad) l = NAN;
+        if (FEW) {
+#pragma unroll
+            for (int k = 0; k < S::NO / 2; k++) {
+                o[k].x += __shfl_xor_sync(FULL, o[k].x, 16);
+                o[k].y += __shfl_xor_sync(FULL, o[k].y, 16);
+            }
+        }
     }
     // outputs e .. e + 3 of chunk group k: element d of the head
     __device__ __forceinline__ static int element(int k, int e) {
@@ -498,7 +520,7 @@ __device__ __forceinline__ int tile_heads(const PagedArgs& A, int unit, int* hea
 }
 
 // Short sequences: one CTA per unit, its warps take every fourth step and meet in shared memory.
-template <int TYPE, int D>
+template <int TYPE, int D, bool FEW>
 __global__ void __launch_bounds__(PG_THREADS, PG_CTAS) k_paged_unit(const PagedArgs A) {
     using S = Shape<TYPE, D>;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -527,7 +549,7 @@ __global__ void __launch_bounds__(PG_THREADS, PG_CTAS) k_paged_unit(const PagedA
     };
 #pragma unroll
     for (int s = 0; s < PG_STAGES - 1; s++) issue(s);
-    Tile<TYPE, D> tile;
+    Tile<TYPE, D, FEW> tile;
     tile.start(A, c);
     int stage = 0;
     for (c.i = warp; c.i < c.sp.steps; c.i += PG_WARPS) {
@@ -574,7 +596,7 @@ __global__ void __launch_bounds__(PG_THREADS, PG_CTAS) k_paged_unit(const PagedA
 
 // Warp w of the launch takes the steps [w per, (w + 1) per) of the line, whatever units they belong to; the loads run
 // ahead of the products across the units' ends.
-template <int TYPE, int D>
+template <int TYPE, int D, bool FEW>
 __global__ void __launch_bounds__(PG_THREADS, PG_CTAS) k_paged_line(const PagedArgs A) {
     using S = Shape<TYPE, D>;
     extern __shared__ __align__(16) uint8_t smem[];
@@ -673,7 +695,7 @@ __global__ void __launch_bounds__(PG_THREADS, PG_CTAS) k_paged_line(const PagedA
     };
 #pragma unroll
     for (int s = 0; s < PG_STAGES - 1; s++) issue(s);
-    Tile<TYPE, D> tile;
+    Tile<TYPE, D, FEW> tile;
     int stage = 0;
     do {
         const int i0 = c.i, steps = static_cast<int>(min(static_cast<long long>(c.sp.steps - c.i), hi - c.pos));
@@ -844,7 +866,7 @@ __global__ void __launch_bounds__(256) k_paged_join(const PagedArgs A, int warps
     }
 }
 
-template <int TYPE, int D>
+template <int TYPE, int D, bool FEW>
 int launch(const PagedArgs& A, bool split, unsigned grid, cudaStream_t st) {
     constexpr int smem = Shape<TYPE, D>::SMEM;
     static unsigned long long devs_set = 0;
@@ -852,24 +874,24 @@ int launch(const PagedArgs& A, bool split, unsigned grid, cudaStream_t st) {
     if (cudaGetDevice(&dev) != cudaSuccess) return -1;
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(__atomic_load_n(&devs_set, __ATOMIC_ACQUIRE) & bit)) {
-        if (cudaFuncSetAttribute(k_paged_line<TYPE, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-            cudaFuncSetAttribute(k_paged_unit<TYPE, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        if (cudaFuncSetAttribute(k_paged_line<TYPE, D, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+            cudaFuncSetAttribute(k_paged_unit<TYPE, D, FEW>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
             return -1;
         __atomic_fetch_or(&devs_set, bit, __ATOMIC_RELEASE);
     }
-    if (!split) return kx::launch_pdl(k_paged_unit<TYPE, D>, dim3(grid), dim3(PG_THREADS), smem, st, A);
-    if (kx::launch_pdl(k_paged_line<TYPE, D>, dim3(grid), dim3(PG_THREADS), smem, st, A) != 0) return -1;
+    if (!split) return kx::launch_pdl(k_paged_unit<TYPE, D, FEW>, dim3(grid), dim3(PG_THREADS), smem, st, A);
+    if (kx::launch_pdl(k_paged_line<TYPE, D, FEW>, dim3(grid), dim3(PG_THREADS), smem, st, A) != 0) return -1;
     return kx::launch_pdl(k_paged_join, dim3(grid), dim3(256), 0, st, A, static_cast<int>(grid * PG_WARPS));
 }
 
 // D: the head dims rounded up to 32; every size runs without a branch inside a step
-template <int TYPE>
+template <int TYPE, bool FEW>
 int launch_d(const PagedArgs& A, bool split, unsigned grid, cudaStream_t st) {
     switch ((std::max(A.c.dk, A.c.dv) + 31) / 32) {
-        case 1: return launch<TYPE, 32>(A, split, grid, st);
-        case 2: return launch<TYPE, 64>(A, split, grid, st);
-        case 3: return launch<TYPE, 96>(A, split, grid, st);
-        default: return launch<TYPE, 128>(A, split, grid, st);
+        case 1: return launch<TYPE, 32, FEW>(A, split, grid, st);
+        case 2: return launch<TYPE, 64, FEW>(A, split, grid, st);
+        case 3: return launch<TYPE, 96, FEW>(A, split, grid, st);
+        default: return launch<TYPE, 128, FEW>(A, split, grid, st);
     }
 }
 
@@ -925,9 +947,9 @@ int kx_attention_paged(const kx_kv* c, int layer, const float* q, int ldq, int H
     const bool split = (keys + ks - 1) / ks > PG_UNIT_STEPS;
     const unsigned grid = split ? std::min(PG_CTAS * sms, PG_MAX_WARPS / PG_WARPS) : static_cast<unsigned>(units);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (c->type == KX_KV_F32) return launch_d<KX_KV_F32>(A, split, grid, st);
-    if (c->type == KX_KV_F16) return launch_d<KX_KV_F16>(A, split, grid, st);
-    return launch_d<KX_KV_BF16>(A, split, grid, st);
+    if (c->type == KX_KV_F32) return launch_d<KX_KV_F32, false>(A, split, grid, st);
+    if (c->type == KX_KV_F16) return launch_d<KX_KV_F16, false>(A, split, grid, st);
+    return A.per_chunk <= 4 ? launch_d<KX_KV_BF16, true>(A, split, grid, st) : launch_d<KX_KV_BF16, false>(A, split, grid, st);
 }
 
 }  // extern "C"
