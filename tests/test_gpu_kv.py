@@ -239,6 +239,21 @@ def test_compact(kx, n_pages, layers, inner, dtype):
         p.check()
 
 
+def test_without_a_status_word_and_on_the_default_stream(kx):
+    p = Pair(kx, 4, 3, 5, 4)
+    want, granted = p.ints([9, 9, 9, 1]), p.ints([0] * 4)
+    seqs, src, dst = p.ints([0, 9, 0]), p.ints([1, 1]), p.ints([0, 1])
+    torch.cuda.synchronize()
+    kx.call("kx_kv_extend", ref(p.c), want.data_ptr(), granted.data_ptr(), *p.w(), None, None)
+    kx.call("kx_kv_free", ref(p.c), seqs.data_ptr(), 3, None, None)
+    kx.call("kx_kv_fork", ref(p.c), src.data_ptr(), dst.data_ptr(), 2, *p.w(), None, None)
+    assert np.array_equal(p.m.extend(want.cpu().numpy()), granted.cpu().numpy())
+    p.m.free([0, 9, 0])
+    p.m.fork(np.array([1, 1]), np.array([0, 1]))
+    p.m.status = 0
+    p.check()
+
+
 def test_turnover_captured_in_a_graph(kx):
     """a step of free, extend, append and fork, captured once and replayed on changing requests"""
     p = Pair(kx, 16, 8, 90, 4, heads=2, dk=16, dv=16, dtype="bf16")

@@ -178,6 +178,52 @@ def test_rows_name_their_slots(kx):
     assert bool((ctx[[1, 6]] == 7).all()) and bool(ctx[[5, 7]].isnan().all()) and int(c.status) == BAD_REQUEST
 
 
+def test_rows_name_their_slots_in_a_split_launch(kx):
+    c = Case([3000, 0, 700], 2, 3, 64, 64, 8, "bf16")
+    seqs = torch.tensor([-1, 2, -1, 0, 5, 1, 2, -9, -1], dtype=torch.int32, device="cuda")
+    q = torch.randn(9, 384, generator=torch.Generator().manual_seed(8))
+    ctx = c.run(kx, q=q, seqs=seqs)
+    c.check(ctx, rows=[(1, 2), (3, 0), (5, 1), (6, 2)], q=q)
+    assert bool((ctx[[0, 2, 7, 8]] == 7).all()) and bool(ctx[4].isnan().all()) and int(c.status) == BAD_REQUEST
+    ctx = c.run(kx, q=q, seqs=torch.full_like(seqs, -1))
+    assert bool((ctx == 7).all())
+
+
+@pytest.mark.parametrize("page", [2, 1024])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_smallest_and_largest_pages(kx, page, dtype):
+    c = Case([1, 1500, 1024, 1025, 2], 2, 2, 32, 40, page, dtype, window=300, sinks=5)
+    c.check(c.run(kx))
+
+
+def test_layers_inside_a_page(kx):
+    c = Case([90, 33], 2, 4, 64, 48, 16, "f16", layers=3, layer=1)
+    for x in ("k", "v"):
+        setattr(c, x, getattr(c, x).transpose(0, 1).contiguous().transpose(0, 1))
+    c.check(c.run(kx))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_split_launch_captured(kx, dtype):
+    """replays follow the lengths, which are device memory"""
+    c = Case([6000, 100, 2000], 2, 4, 64, 64, 16, dtype, seed=6)
+    c.run(kx)
+    cc, qd, ctx = c.cache(kx), c.q.cuda(), torch.zeros(3, 512, device="cuda")
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        kx.call("kx_attention_paged", ref(cc), 0, qd.data_ptr(), 512, 8, None, 3, 0, 0, 0.0, ctx.data_ptr(), 512, c.ws.data_ptr(),
+                c.ws.numel(), None, torch.cuda.current_stream().cuda_stream)
+    for lens in ([6000, 100, 2000], [5, 99, 1999], [0, 0, 1], [5999, 1, 0]):
+        c.d_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        short = Case.__new__(Case)
+        short.__dict__.update(c.__dict__)
+        short.lens, short.host = lens, [(k[:n], v[:n]) for (k, v), n in zip(c.host, lens)]
+        short.check(ctx)
+
+
 @pytest.mark.parametrize("long", [False, True])
 def test_bad_pages_and_lengths_give_nan_rows(kx, long):
     n = 5000 if long else 60
