@@ -66,7 +66,9 @@ struct WinArgs {
     int G, chunks, per_chunk;  // query heads per key-value head, groups of them, heads per group (<= 128)
     int tiles;                 // of 64 keys in S
     int ka, vp;                // K planes of 64 x 64; value columns rounded up to 16
-    int qt, qtiles;            // queries per CTA, CTAs per sample and group
+    int qt, qtiles;            // queries per block of rows, blocks per sample and group
+    int splits;                // CTAs per block of rows, each with a part of its tiles
+    size_t parts;              // where in the workspace their results are
     uint32_t block;            // bytes per tile of the workspace
     float scale2;
     bool vecq, veck, vecv;
@@ -97,6 +99,26 @@ struct Tiles {
     __device__ __forceinline__ int count() const { return na + end - b0; }
     __device__ __forceinline__ int at(int i) const { return i < na ? i : b0 + i - na; }
 };
+// a block of WN_ROWS rows: queries i0 .. of a sample, the heads of a group
+struct Block {
+    int b, kvh, head0, heads, i0;
+    __device__ __forceinline__ Block(const WinArgs& A, int index) {  // later queries see more keys: they come first
+        const int per = A.B * A.Hkv * A.chunks, x = index % per, chunk = x % A.chunks, bh = x / A.chunks;
+        b = bh / A.Hkv;
+        kvh = bh - b * A.Hkv;
+        head0 = kvh * A.G + chunk * A.per_chunk;
+        heads = min(A.per_chunk, A.G - chunk * A.per_chunk);
+        i0 = (A.qtiles - 1 - index / per) * A.qt;
+    }
+};
+// A CTA's part of a split block: per row maximum and sum, then the rows' outputs, not divided yet; the first CTA's also
+// says whether there is something to join.
+constexpr int WN_MAX_PARTS = 224;
+struct alignas(16) PartHead {
+    int join, pad[3];
+    float2 ml[WN_ROWS];
+};
+__host__ __device__ inline size_t part_bytes(int dv) { return sizeof(PartHead) + static_cast<size_t>(WN_ROWS) * ((dv + 3) / 4 * 4) * 4; }
 __device__ __forceinline__ Tiles tiles_of(const WinArgs& A, int p0, int p1) {
     Tiles t{0, 0, 0};
     if (p1 < 0) return t;
@@ -280,18 +302,17 @@ __device__ __noinline__ void plain_rows(const WinArgs& A, int b, int kvh, int he
     }
 }
 
-template <int D>
+// SPLIT: a block's tiles over A.splits CTAs
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constant__ WinArgs A) {
     using W = Win<D>;
     extern __shared__ uint8_t smem_raw[];
     __shared__ WinCtl ctl;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // later queries see more keys: their CTAs first
-    const int per = A.B * A.Hkv * A.chunks;
-    const int qi = A.qtiles - 1 - static_cast<int>(blockIdx.x) / per, x = static_cast<int>(blockIdx.x) % per;
-    const int chunk = x % A.chunks, bh = x / A.chunks, b = bh / A.Hkv, kvh = bh - b * A.Hkv;
-    const int head0 = kvh * A.G + chunk * A.per_chunk, heads = min(A.per_chunk, A.G - chunk * A.per_chunk);
+    const int splits = SPLIT ? A.splits : 1, block = static_cast<int>(blockIdx.x) / splits, split = static_cast<int>(blockIdx.x) - block * splits;
+    const Block at(A, block);
+    const int b = at.b, kvh = at.kvh, head0 = at.head0, heads = at.heads, i0 = at.i0, bh = b * A.Hkv + kvh;
 
     if (tid == 0) {
         for (int s = 0; s < 3; s++) {
@@ -323,10 +344,11 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     kx::tc_fence_after();
     const uint32_t tmem = ctl.tmem;
     kx::griddep_wait();
+    if (SPLIT) kx::griddep_launch_dependents();
 
     int ql, kl;
     const bool lens_ok = sample_lens(A, b, &ql, &kl);
-    const int i0 = qi * A.qt, nq = lens_ok ? max(0, min(A.qt, ql - i0)) : 0, rows = nq * heads, off = kl - ql;
+    const int nq = lens_ok ? max(0, min(A.qt, ql - i0)) : 0, rows = nq * heads, off = kl - ql;
     if (!lens_ok) {  // NaN rows, reported
         if (tid == 0) kx::kv_report(A.status, KX_STATUS_BAD_REQUEST);
         const int nr = min(A.qt, A.Rq - i0);
@@ -337,7 +359,10 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     }
     Tiles tl{0, 0, 0};
     if (nq > 0) tl = tiles_of(A, off + i0, off + i0 + nq - 1);
-    const int n_tiles = tl.count();
+    const int all_tiles = tl.count(), t0 = static_cast<int>(static_cast<long>(all_tiles) * split / splits);
+    const int n_tiles = static_cast<int>(static_cast<long>(all_tiles) * (split + 1) / splits) - t0;
+    const auto tile_at = [&](int t) { return tl.at(t0 + t); };
+    PartHead* part = reinterpret_cast<PartHead*>(A.ws + A.parts + blockIdx.x * part_bytes(A.dv));
     const uint8_t* blocks = A.ws + static_cast<size_t>(bh) * A.tiles * A.block;
     const TileInfo* info = infos(A) + static_cast<size_t>(bh) * A.tiles;
 
@@ -346,14 +371,14 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
         const int s = t % 3;
         if (t >= 3 && !kx::mbar_wait(&ctl.kfree[s], (t / 3 - 1) & 1, &ctl.abort, A.status)) return false;
         kx::mbar_arrive_expect_tx(&ctl.kfull[s], k_bytes(A.ka));
-        kx::bulk_load(smem + W::k_at(s), blocks + static_cast<size_t>(tl.at(t)) * A.block, k_bytes(A.ka), &ctl.kfull[s]);
+        kx::bulk_load(smem + W::k_at(s), blocks + static_cast<size_t>(tile_at(t)) * A.block, k_bytes(A.ka), &ctl.kfull[s]);
         return true;
     };
     const auto fetch_v = [&](int t) {
         const int s = t % 3;
         if (t >= 3 && !kx::mbar_wait(&ctl.vfree[s], (t / 3 - 1) & 1, &ctl.abort, A.status)) return false;
         kx::mbar_arrive_expect_tx(&ctl.vfull[s], v_bytes(A.vp));
-        kx::bulk_load(smem + W::v_at(s), blocks + static_cast<size_t>(tl.at(t)) * A.block + k_bytes(A.ka), v_bytes(A.vp), &ctl.vfull[s]);
+        kx::bulk_load(smem + W::v_at(s), blocks + static_cast<size_t>(tile_at(t)) * A.block + k_bytes(A.ka), v_bytes(A.vp), &ctl.vfull[s]);
         return true;
     };
     constexpr int EARLY = 2;  // tiles fetched while q is prepared (K's third place is lent to q until then)
@@ -389,7 +414,7 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
             i += di, h += dh;
             if (h >= heads) h -= heads, i++;
         }
-        for (int t = tid; t < n_tiles; t += 2 * WN_GROUP) slow = slow || __ldcg(&info[tl.at(t)].plain) != 0;
+        for (int t = tid; t < all_tiles; t += 2 * WN_GROUP) slow = slow || __ldcg(&info[tl.at(t)].plain) != 0;
         asm volatile("cp.async.wait_all;" ::: "memory");
         kx::named_bar(1, 2 * WN_GROUP);
         float4 f[D / 8];
@@ -426,7 +451,8 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     kx::tc_fence_after();
     const bool slow = ctl.slow != 0;
     const int n = slow ? 0 : n_tiles;
-    if (slow && grp < 2) plain_rows(A, b, kvh, head0, heads, i0, rows, off, warp, 8);
+    if (SPLIT && tid == 0 && split == 0) part->join = !slow && all_tiles > 0;
+    if (slow && grp < 2 && split == 0) plain_rows(A, b, kvh, head0, heads, i0, rows, off, warp, 8);
 
     if (grp == 2) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -518,7 +544,7 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
         const uint32_t om = tmem + lanes + W::TO + grp * D;
         const int p_first = off + i0, p_last = off + i0 + nq - 1;
         float2 scales = make_float2(1.0f, 1.0f);  // a tile's, fetched a tile ahead
-        if (grp < n) scales = __ldcg(reinterpret_cast<const float2*>(info + tl.at(grp)));
+        if (grp < n) scales = __ldcg(reinterpret_cast<const float2*>(info + tile_at(grp)));
         float keep = 1.0f, keep_next = 1.0f;
         const auto join = [&](int t) {  // P.V of tile t joins the output
             if (!__all_sync(FULL, kx::mbar_wait(&ctl.ofull[grp], (t / 2) & 1, &ctl.abort, A.status))) return false;
@@ -540,11 +566,11 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
         for (int t = grp; grp < n; t += 2) {
             if (t < n) {  // P of tile t
                 const uint32_t sm = tmem + lanes + W::TS + (t % W::NS) * WN_KEYS;
-                const int j0 = tl.at(t) * WN_KEYS;
+                const int j0 = tile_at(t) * WN_KEYS;
                 const float f = fmaxf(cs * scales.x, 1.17549435e-38f);  // positive: -inf stays -inf
                 const float shrink = unit * (1.0f / scales.y);           // powers of two
                 unit = scales.y;
-                if (t + 2 < n) scales = __ldcg(reinterpret_cast<const float2*>(info + tl.at(t + 2)));
+                if (t + 2 < n) scales = __ldcg(reinterpret_cast<const float2*>(info + tile_at(t + 2)));
                 if (!__all_sync(FULL, kx::mbar_wait(&ctl.sfull[t % W::NS], (t / W::NS) & 1, &ctl.abort, A.status))) break;
                 kx::tc_fence_after();
                 float alpha;
@@ -621,7 +647,9 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                 const float* his = ml + ((grp ^ 1) * WN_ROWS + r) * 3;
                 const float mm = fmaxf(m, his[0]), safe = mm == -INFINITY ? 0.0f : mm;
                 float f0 = kx::ex2_approx(m - safe), f1 = kx::ex2_approx(his[0] - safe);
-                const float den = f0 * l + f1 * his[1], inv = den == 0.0f ? 0.0f : 1.0f / den;
+                const float den = f0 * l + f1 * his[1];
+                if (SPLIT && grp == 0) part->ml[r] = make_float2(mm, den);
+                const float inv = SPLIT ? 1.0f : den == 0.0f ? 0.0f : 1.0f / den;
                 f0 *= inv * unit, f1 *= inv * his[2];
                 float* z = half + (grp * WN_ROWS + r) * P;
 #pragma unroll
@@ -635,14 +663,17 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
             const int di = 8 / heads, dh = 8 - di * heads;
             int i = warp / heads, h = warp - i * heads;
             for (int x = warp; x < rows && !ctl.abort; x += 8) {
-                float* out = A.ctx + (static_cast<long>(b) * A.Rq + i0 + i) * A.ldc + static_cast<long>(head0 + h) * A.dv;
+                float* out = SPLIT ? reinterpret_cast<float*>(part + 1) + x * ((A.dv + 3) / 4 * 4)
+                                          : A.ctx + (static_cast<long>(b) * A.Rq + i0 + i) * A.ldc + static_cast<long>(head0 + h) * A.dv;
 #pragma unroll
                 for (int c = 0; c < D; c += 32)
                     if (c + lane < A.dv) out[c + lane] = half[(c < D / 2 ? 0 : WN_ROWS * P) + x * P + c % (D / 2) + lane];
                 i += di, h += dh;
                 if (h >= heads) h -= heads, i++;
             }
-        } else if (!slow && grp == 0 && r < rows) {  // rows that see nothing
+        } else if (SPLIT && !slow && all_tiles > 0) {  // a split block with fewer tiles than parts
+            if (grp == 0) part->ml[r] = make_float2(-INFINITY, 0.0f);
+        } else if (!slow && split == 0 && grp == 0 && r < rows) {  // rows that see nothing
             float* out = A.ctx + (static_cast<long>(b) * A.Rq + i0 + my_i) * A.ldc + static_cast<long>(head0 + r % heads) * A.dv;
             for (int y = 0; y < A.dv; y++) out[y] = 0.0f;
         }
@@ -655,10 +686,61 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     }
 }
 
+// CTA (block, quarter): 32 rows of a split block out of its parts, a warp per row and four elements per lane, the parts in
+// their order, eight at a time.
+__global__ void __launch_bounds__(256) k_win_join(const __grid_constant__ WinArgs A) {
+    kx::griddep_wait();
+    kx::griddep_launch_dependents();
+    const int block = blockIdx.x >> 2, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pitch = (A.dv + 3) / 4 * 4;
+    const size_t bytes = part_bytes(A.dv);
+    const uint8_t* parts = A.ws + A.parts + static_cast<size_t>(block) * A.splits * bytes;
+    if (!__ldcg(&reinterpret_cast<const PartHead*>(parts)->join)) return;
+    const Block at(A, block);
+    int ql, kl;
+    if (!sample_lens(A, at.b, &ql, &kl)) return;
+    const int rows = min(A.qt, ql - at.i0) * at.heads;
+    for (int r = (blockIdx.x & 3) * 32 + warp; r < min(rows, ((blockIdx.x & 3) + 1) * 32); r += 8) {
+        float m = -INFINITY, den = 0.0f;
+        float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s0 = 0; s0 < A.splits; s0 += 8) {
+            float2 ml[8];
+            float4 v[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const PartHead* p = reinterpret_cast<const PartHead*>(parts + min(s0 + u, A.splits - 1) * bytes);
+                ml[u] = s0 + u < A.splits ? __ldcg(&p->ml[r]) : make_float2(-INFINITY, 0.0f);
+                v[u] = lane * 4 < pitch ? __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p + 1) + r * pitch + lane * 4))
+                                        : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            float top = m;
+#pragma unroll
+            for (int u = 0; u < 8; u++) top = fmaxf(top, ml[u].x);
+            const float safe = top == -INFINITY ? 0.0f : top, back = kx::ex2_approx(m - safe);
+            m = top;
+            den *= back;
+            num.x *= back, num.y *= back, num.z *= back, num.w *= back;
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                if (ml[u].x == -INFINITY) continue;  // that part saw nothing of the row: its output may not be there
+                const float f = kx::ex2_approx(ml[u].x - safe);
+                den += f * ml[u].y;
+                num.x += f * v[u].x, num.y += f * v[u].y, num.z += f * v[u].z, num.w += f * v[u].w;
+            }
+        }
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+        const int i = r / at.heads, h = r - i * at.heads;
+        float* out = A.ctx + (static_cast<long>(at.b) * A.Rq + at.i0 + i) * A.ldc + static_cast<long>(at.head0 + h) * A.dv;
+        const float z[4] = {num.x * inv, num.y * inv, num.z * inv, num.w * inv};
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (lane * 4 + e < A.dv) out[lane * 4 + e] = z[e];
+    }
+}
+
 struct WinLayout {
     int tiles, ka, vp;
     uint32_t block;
-    size_t bytes;
+    size_t parts, bytes;
 };
 bool layout_of(int B, int S, int Hkv, int dk, int dv, WinLayout* L) {
     if (B < 0 || S < 1 || Hkv < 1 || dk < 1 || dv < 1 || dk > WN_DMAX || dv > WN_DMAX || S > INT32_MAX - 256) return false;
@@ -668,7 +750,8 @@ bool layout_of(int B, int S, int Hkv, int dk, int dv, WinLayout* L) {
     L->block = k_bytes(L->ka) + v_bytes(L->vp);
     const double blocks = static_cast<double>(B) * Hkv * L->tiles;
     if (blocks > 2e9) return false;
-    L->bytes = static_cast<size_t>(B) * Hkv * L->tiles * (L->block + sizeof(TileInfo));
+    L->parts = (static_cast<size_t>(B) * Hkv * L->tiles * (L->block + sizeof(TileInfo)) + 127) / 128 * 128;
+    L->bytes = L->parts + WN_MAX_PARTS * part_bytes(dv);
     return true;
 }
 
@@ -689,11 +772,11 @@ int launch_prep(const WinArgs& A, unsigned grid, cudaStream_t st) {
     return kx::launch_pdl(k_win_prep, dim3(grid), dim3(256), WN_PREP_SMEM, st, A);
 }
 
-template <int D>
+template <int D, bool SPLIT>
 int launch_main(const WinArgs& A, unsigned grid, cudaStream_t st) {
     static unsigned long long devs_set = 0;
-    if (allow_smem(reinterpret_cast<const void*>(k_win_main<D>), Win<D>::SMEM, &devs_set) != 0) return -1;
-    return kx::launch_pdl(k_win_main<D>, dim3(grid), dim3(WN_THREADS), Win<D>::SMEM, st, A);
+    if (allow_smem(reinterpret_cast<const void*>(k_win_main<D, SPLIT>), Win<D>::SMEM, &devs_set) != 0) return -1;
+    return kx::launch_pdl(k_win_main<D, SPLIT>, dim3(grid), dim3(WN_THREADS), Win<D>::SMEM, st, A);
 }
 
 }  // namespace
@@ -732,11 +815,24 @@ int kx_attention_window(const float* q, int ldq, const float* k, int ldk, const 
     A.scale2 = (scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(dk)) : scale) * 1.4426950408889634f;
     const auto vec = [](const float* p, int ld, int d) { return ((ld | d) & 3) == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     A.vecq = vec(q, ldq, dk), A.veck = vec(k, ldk, dk), A.vecv = vec(v, ldv, dv);
-    const double grid = static_cast<double>(A.qtiles) * B * Hkv * A.chunks;
-    if (grid > 2e9) return -1;
+    const double blocks = static_cast<double>(A.qtiles) * B * Hkv * A.chunks;
+    if (blocks > 2e9) return -1;
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
+        return -1;
+    // Two CTAs and more per block of rows where SMs would be idle otherwise: its tiles in as many parts, joined by a third
+    // launch, at least four tiles (8 us) to a CTA. (Two parts each for 102 blocks on 148 SMs took 73 us against 58.)
+    const int grid = static_cast<int>(blocks);
+    const long reach = A.window > 0 ? std::min(static_cast<long>(S), static_cast<long>(A.window) + A.qt + A.sinks + 2 * WN_KEYS) : S;
+    A.splits = static_cast<int>(std::min(static_cast<long>(sms / grid), reach / (4 * WN_KEYS)));
+    if (A.splits < 2 || static_cast<long>(A.splits) * grid > WN_MAX_PARTS) A.splits = 1;
+    A.parts = L.parts;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (launch_prep(A, static_cast<unsigned>(B * Hkv * L.tiles), st) != 0) return -1;
-    return dk <= 64 && dv <= 64 ? launch_main<64>(A, static_cast<unsigned>(grid), st) : launch_main<128>(A, static_cast<unsigned>(grid), st);
+    const bool small = dk <= 64 && dv <= 64;
+    if (A.splits == 1) return small ? launch_main<64, false>(A, grid, st) : launch_main<128, false>(A, grid, st);
+    if ((small ? launch_main<64, true>(A, grid * A.splits, st) : launch_main<128, true>(A, grid * A.splits, st)) != 0) return -1;
+    return kx::launch_pdl(k_win_join, dim3(static_cast<unsigned>(grid) * 4), dim3(256), 0, st, A);
 }
 
 }  // extern "C"

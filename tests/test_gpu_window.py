@@ -141,6 +141,39 @@ def test_long(kx, window, sinks, Rq):
     assert torch.equal(again, c.ctx)
 
 
+@pytest.mark.parametrize("B,Rq,S,H,Hkv,dk,dv,window,sinks", [
+    (1, 1, 5000, 1, 1, 64, 64, 0, 0), (1, 1, 3000, 8, 2, 128, 128, 0, 0), (2, 129, 4000, 2, 2, 64, 50, 0, 0),
+    (1, 100, 4000, 3, 1, 128, 33, 1500, 7), (3, 300, 1100, 6, 2, 80, 72, 0, 0), (1, 40, 2500, 140, 1, 32, 32, 0, 0)])
+def test_few_rows_over_many_keys(kx, B, Rq, S, H, Hkv, dk, dv, window, sinks):
+    """blocks of rows whose keys are split over several CTAs"""
+    c = Case(B, Rq, S, H, Hkv, dk, dv, window, sinks, seed=S)
+    ctx = c.run(kx).clone()
+    c.check(ctx)
+    c.launch(kx, sp())
+    torch.cuda.synchronize()
+    assert torch.equal(ctx, c.ctx)
+
+
+def test_split_blocks_of_all_kinds(kx):
+    """some with a few keys, some without any, a bad sample, one with values that parts cannot hold"""
+    c = Case(5, 60, 2000, 2, 1, 64, 64, q_len=[60, 60, 30, 0, 60], k_len=[2000, 70, 7, 5, 1900], pad=3)
+    c.k[4, 1000, 0, 3] = float("nan")
+    c.args(kx)
+    c.launch(kx, sp())
+    torch.cuda.synchronize()
+    ctx = c.ctx[:, :128]
+    c.k[4, 1000, 0, 3] = 0
+    assert bool(ctx[240:300].isnan().all())
+    c.ctx[240:300, :128] = float("nan")
+    c.check(c.ctx, samples=[0, 1, 2, 3])
+    c.lens[1][0] = 2001
+    c.launch(kx, sp())
+    torch.cuda.synchronize()
+    assert bool(c.ctx[:60, :128].isnan().all()) and int(c.status) == BAD_REQUEST
+    c.ctx[:60, :128] = 0
+    c.check(c.ctx, samples=[1, 2, 3])
+
+
 @pytest.mark.parametrize("pad", [1, 3, 4])
 def test_row_pitches(kx, pad):
     c = Case(2, 70, 130, 4, 2, 64, 48, 50, 2, pad=pad)
