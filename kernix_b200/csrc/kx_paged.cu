@@ -45,11 +45,18 @@ constexpr int PG_STAGES = 3;
 constexpr int PG_CTAS = 2;        // per SM (three, with registers for each, measured up to 10 % slower)
 constexpr int PG_HEADS = 8;       // query heads per tile
 constexpr int PG_MAX_WARPS = 1280;  // of a launch over the line: sizes the workspace
-constexpr int PG_MIN_STEPS = 4;     // a warp's range is at least this many steps: a part more costs as much as a few
+// a warp's range is at least this long: one row of 640 keys took 9.7 us with 2, 12.5 with 4, 15.8 with 8
+constexpr int PG_MIN_STEPS = 2;
 // a unit's place on the line before its steps: its q, its output (32 ragged bf16 rows: 26.7 us with 1, 24.7 with 3,
 // 27.7 with 6)
 constexpr int PG_UNIT_COST = 3;
-constexpr int PG_UNIT_STEPS = 24;   // a unit of at most this many steps is one CTA's
+// Units of few steps at most get a CTA each, which joins its warps itself: 5.8 us for 12 steps of 4 units where the line
+// and its join take 11. Whether lengths are near their bound is not known here, so the bound grows with the units: 40 steps
+// of 64 units 13.1 us against 14.2, of 4 units 12.2 against 9.7; 80 steps of 800 units 84 us against 97, of 64 units 22
+// against 19.
+inline bool pg_by_units(long steps, long units, int sms) {
+    return steps <= 32 || (steps <= 48 && units >= 64) || (steps <= 96 && units >= 4l * sms);
+}
 constexpr int PG_DMAX = 128;
 
 struct PagedArgs {
@@ -940,11 +947,11 @@ int kx_attention_paged(const kx_kv* c, int layer, const float* q, int ldq, int H
         return -1;
     const long units = static_cast<long>(n) * c->heads * A.chunks;
     if (units > INT32_MAX) return -1;
-    // the most steps a unit can have: few enough for one CTA, which then needs no join
+    // the most steps a unit can have
     const int ks = c->type == KX_KV_F32 ? 8 : 16;
     long keys = static_cast<long>(c->max_pages) * c->page;
     if (window > 0) keys = std::min(keys, static_cast<long>(window) + sinks + 2 * ks);
-    const bool split = (keys + ks - 1) / ks > PG_UNIT_STEPS;
+    const bool split = !pg_by_units((keys + ks - 1) / ks, units, sms);
     const unsigned grid = split ? std::min(PG_CTAS * sms, PG_MAX_WARPS / PG_WARPS) : static_cast<unsigned>(units);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (c->type == KX_KV_F32) return launch_d<KX_KV_F32, false>(A, split, grid, st);

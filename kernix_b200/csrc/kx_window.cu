@@ -310,7 +310,8 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     __shared__ WinCtl ctl;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int splits = SPLIT ? A.splits : 1, block = static_cast<int>(blockIdx.x) / splits, split = static_cast<int>(blockIdx.x) - block * splits;
+    const int splits = SPLIT ? A.splits : 1;
+    const int block = static_cast<int>(blockIdx.x) / splits, split = static_cast<int>(blockIdx.x) - block * splits;
     const Block at(A, block);
     const int b = at.b, kvh = at.kvh, head0 = at.head0, heads = at.heads, i0 = at.i0, bh = b * A.Hkv + kvh;
 
@@ -320,8 +321,6 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
             kx::mbar_init(&ctl.kfree[s], 1);
             kx::mbar_init(&ctl.sfull[s], 1);
             kx::mbar_init(&ctl.sfree[s], 1);
-        }
-        for (int s = 0; s < 3; s++) {
             kx::mbar_init(&ctl.vfull[s], 1);
             kx::mbar_init(&ctl.vfree[s], 1);
         }
@@ -406,7 +405,8 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
             float4* to = stage + x * (D / 4) + (y ^ (x & 7));
             if (A.vecq) {
                 const bool in = x < rows && y * 4 < A.dk;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(kx::smem_u32(to)), "l"(in ? qr + y * 4 : A.q), "r"(in ? 16 : 0)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                             ::"r"(kx::smem_u32(to)), "l"(in ? qr + y * 4 : A.q), "r"(in ? 16 : 0)
                              : "memory");
             } else {
                 *to = x < rows ? load4(qr, y * 4, A.dk, false) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
             // no copy may be under way when the CTA ends; where everything went well its last reader has seen to that
             if (slow || !good || ctl.abort) {
                 const uint64_t t0 = kx::globaltimer();
-                                uint64_t* full = warp == 8 ? ctl.kfull : ctl.vfull;
+                uint64_t* full = warp == 8 ? ctl.kfull : ctl.vfull;
                 for (int t = max(0, sent - 3); t < sent; t++)
                     while (!kx::mbar_try_wait(&full[t % 3], (t / 3) & 1) && kx::globaltimer() - t0 < KX_WAIT_NS) __nanosleep(256);
             }
@@ -607,7 +607,8 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int y = 0; y < 32; y += 2) {
-                        float2 e = kx::fma2(make_float2(__uint_as_float(x[y]), __uint_as_float(x[y + 1])), make_float2(f, f), make_float2(shift, shift));
+                        float2 e = kx::fma2(make_float2(__uint_as_float(x[y]), __uint_as_float(x[y + 1])), make_float2(f, f),
+                                            make_float2(shift, shift));
                         e.x = kx::ex2_approx(e.x);
                         e.y = kx::ex2_approx(e.y);
                         sum[y / 2 & 1] = kx::add2(sum[y / 2 & 1], e);

@@ -128,7 +128,8 @@ def test_ragged_rows(kx, dtype, shape):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("lens,window,sinks", [([20000], 0, 0), ([1, 30011, 5], 0, 0), ([40000, 39999], 20001, 9), ([257] * 300, 0, 0)])
+@pytest.mark.parametrize("lens,window,sinks", [([20000], 0, 0), ([1, 30011, 5], 0, 0), ([40000, 39999], 20001, 9), ([257] * 300, 0, 0),
+                                               ([30, 0] * 100 + [9000, 1], 0, 0)])
 def test_long_and_many_rows(kx, dtype, lens, window, sinks):
     """heads split over many CTAs and joined; ranges that cover several rows"""
     c = Case(lens, 2, 4, 128, 128, 32, dtype, window, sinks, seed=3)
