@@ -239,6 +239,24 @@ def test_compact(kx, n_pages, layers, inner, dtype):
         p.check()
 
 
+def test_more_pages_slots_and_pairs_than_one_pass_takes(kx):
+    rng = np.random.default_rng(8)
+    p = Pair(kx, 2600, 40, 70001, 4, heads=1, dk=8, dv=8)
+    p.extend(rng.integers(0, 120, 2600))
+    p.check()
+    ended = rng.permutation(2600)[:1250]
+    p.free(ended.tolist())
+    p.check()
+    parents = np.setdiff1d(np.arange(2600), ended)
+    p.fork(rng.choice(parents, 1200), ended[:1200])
+    p.check()
+    p.free(rng.permutation(2600)[:900].tolist())
+    p.compact()
+    p.check()
+    p.extend(rng.integers(0, 20, 2600))
+    p.check()
+
+
 def test_without_a_status_word_and_on_the_default_stream(kx):
     p = Pair(kx, 4, 3, 5, 4)
     want, granted = p.ints([9, 9, 9, 1]), p.ints([0] * 4)
