@@ -181,11 +181,21 @@ __global__ void __launch_bounds__(256) k_win_prep(const __grid_constant__ WinArg
     float ktop = 0.0f, vtop = 0.0f;
     const float* kr = A.k + (static_cast<long>(b) * A.S + j0) * A.ldk + h * A.dk;
     const float* vr = A.v + (static_cast<long>(b) * A.S + j0) * A.ldv + h * A.dv;
-#pragma unroll 4
-    for (int r = warp; r < WN_KEYS; r += 8) {  // a warp per row; rows behind the last key are zero
-        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 x = r < n ? load4(kr + static_cast<long>(r) * A.ldk, lane * 4, A.dk, A.veck) : zero;
-        const float4 y = r < n ? load4(vr + static_cast<long>(r) * A.ldv, lane * 4, A.dv, A.vecv) : zero;
+    // a warp per row, all of its rows asked for at once; rows behind the last key are zero
+    float4 kx4[WN_KEYS / 8], vx4[WN_KEYS / 8];
+#pragma unroll
+    for (int u = 0; u < WN_KEYS / 8; u++) {
+        const int r = warp + 8 * u;
+        kx4[u] = vx4[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < n) {
+            kx4[u] = load4(kr + static_cast<long>(r) * A.ldk, lane * 4, A.dk, A.veck);
+            vx4[u] = load4(vr + static_cast<long>(r) * A.ldv, lane * 4, A.dv, A.vecv);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < WN_KEYS / 8; u++) {
+        const int r = warp + 8 * u;
+        const float4 x = kx4[u], y = vx4[u];
         good = good && held4(x) && held4(y);
         ktop = top4(ktop, x);
         vtop = top4(vtop, y);
@@ -361,8 +371,9 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     if (nq > 0) tl = tiles_of(A, off + i0, off + i0 + nq - 1);
     const int all_tiles = tl.count(), t0 = static_cast<int>(static_cast<long>(all_tiles) * split / splits);
     const int n_tiles = static_cast<int>(static_cast<long>(all_tiles) * (split + 1) / splits) - t0;
-    const auto tile_at = [&](int t) { return tl.at(t0 + t); };
-    PartHead* part = reinterpret_cast<PartHead*>(A.ws + A.parts + blockIdx.x * part_bytes(A.dv));
+    const int turn = tl.na - t0, before = t0, behind = tl.b0 - turn;  // this CTA's tile t: tl.at(t0 + t)
+    const auto tile_at = [&](int t) { return t + (t < turn ? before : behind); };
+    const auto part = [&] { return reinterpret_cast<PartHead*>(A.ws + A.parts + blockIdx.x * part_bytes(A.dv)); };
     const uint8_t* blocks = A.ws + static_cast<size_t>(bh) * A.tiles * A.block;
     const TileInfo* info = infos(A) + static_cast<size_t>(bh) * A.tiles;
 
@@ -452,7 +463,7 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     kx::tc_fence_after();
     const bool slow = ctl.slow != 0;
     const int n = slow ? 0 : n_tiles;
-    if (SPLIT && tid == 0 && split == 0) part->join = !slow && all_tiles > 0;
+    if (SPLIT && tid == 0 && split == 0) part()->join = !slow && all_tiles > 0;
     if (slow && grp < 2 && split == 0) plain_rows(A, b, kvh, head0, heads, i0, rows, off, warp, 8);
 
     if (grp == 2) {
@@ -650,7 +661,7 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                 const float mm = fmaxf(m, his[0]), safe = mm == -INFINITY ? 0.0f : mm;
                 float f0 = kx::ex2_approx(m - safe), f1 = kx::ex2_approx(his[0] - safe);
                 const float den = f0 * l + f1 * his[1];
-                if (SPLIT && grp == 0) part->ml[r] = make_float2(mm, den);
+                if (SPLIT && grp == 0) part()->ml[r] = make_float2(mm, den);
                 const float inv = SPLIT ? 1.0f : den == 0.0f ? 0.0f : 1.0f / den;
                 f0 *= inv * unit, f1 *= inv * his[2];
                 float* z = half + (grp * WN_ROWS + r) * P;
@@ -665,7 +676,7 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
             const int di = 8 / heads, dh = 8 - di * heads;
             int i = warp / heads, h = warp - i * heads;
             for (int x = warp; x < rows && !ctl.abort; x += 8) {
-                float* out = SPLIT ? reinterpret_cast<float*>(part + 1) + x * ((A.dv + 3) / 4 * 4)
+                float* out = SPLIT ? reinterpret_cast<float*>(part() + 1) + x * ((A.dv + 3) / 4 * 4)
                                           : A.ctx + (static_cast<long>(b) * A.Rq + i0 + i) * A.ldc + static_cast<long>(head0 + h) * A.dv;
 #pragma unroll
                 for (int c = 0; c < D; c += 32)
@@ -674,7 +685,7 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                 if (h >= heads) h -= heads, i++;
             }
         } else if (SPLIT && !slow && all_tiles > 0) {  // a split block with fewer tiles than parts
-            if (grp == 0) part->ml[r] = make_float2(-INFINITY, 0.0f);
+            if (grp == 0) part()->ml[r] = make_float2(-INFINITY, 0.0f);
         } else if (!slow && split == 0 && grp == 0 && r < rows) {  // rows that see nothing
             float* out = A.ctx + (static_cast<long>(b) * A.Rq + i0 + my_i) * A.ldc + static_cast<long>(head0 + r % heads) * A.dv;
             for (int y = 0; y < A.dv; y++) out[y] = 0.0f;
@@ -688,55 +699,56 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
     }
 }
 
-// CTA (block, quarter): 32 rows of a split block out of its parts, a warp per row and four elements per lane, the parts in
-// their order, eight at a time.
+// A warp per row of a split block, four elements per lane, the block's parts in their order, eight at a time. Everything is
+// asked for before anything is looked at: the launch is one round trip to L2 where the parts are at most eight.
 __global__ void __launch_bounds__(256) k_win_join(const __grid_constant__ WinArgs A) {
     kx::griddep_wait();
     kx::griddep_launch_dependents();
-    const int block = blockIdx.x >> 2, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pitch = (A.dv + 3) / 4 * 4;
+    const int block = blockIdx.x / (WN_ROWS / 8), r = blockIdx.x % (WN_ROWS / 8) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int pitch = (A.dv + 3) / 4 * 4;
     const size_t bytes = part_bytes(A.dv);
     const uint8_t* parts = A.ws + A.parts + static_cast<size_t>(block) * A.splits * bytes;
-    if (!__ldcg(&reinterpret_cast<const PartHead*>(parts)->join)) return;
+    const int wanted = __ldcg(&reinterpret_cast<const PartHead*>(parts)->join);
     const Block at(A, block);
     int ql, kl;
-    if (!sample_lens(A, at.b, &ql, &kl)) return;
-    const int rows = min(A.qt, ql - at.i0) * at.heads;
-    for (int r = (blockIdx.x & 3) * 32 + warp; r < min(rows, ((blockIdx.x & 3) + 1) * 32); r += 8) {
-        float m = -INFINITY, den = 0.0f;
-        float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s0 = 0; s0 < A.splits; s0 += 8) {
-            float2 ml[8];
-            float4 v[8];
+    const bool lens_ok = sample_lens(A, at.b, &ql, &kl);
+    float m = -INFINITY, den = 0.0f;
+    float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < A.splits; s0 += 8) {
+        float2 ml[8];
+        float4 v[8];
 #pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const PartHead* p = reinterpret_cast<const PartHead*>(parts + min(s0 + u, A.splits - 1) * bytes);
-                ml[u] = s0 + u < A.splits ? __ldcg(&p->ml[r]) : make_float2(-INFINITY, 0.0f);
-                v[u] = lane * 4 < pitch ? __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p + 1) + r * pitch + lane * 4))
-                                        : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
-            float top = m;
-#pragma unroll
-            for (int u = 0; u < 8; u++) top = fmaxf(top, ml[u].x);
-            const float safe = top == -INFINITY ? 0.0f : top, back = kx::ex2_approx(m - safe);
-            m = top;
-            den *= back;
-            num.x *= back, num.y *= back, num.z *= back, num.w *= back;
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                if (ml[u].x == -INFINITY) continue;  // that part saw nothing of the row: its output may not be there
-                const float f = kx::ex2_approx(ml[u].x - safe);
-                den += f * ml[u].y;
-                num.x += f * v[u].x, num.y += f * v[u].y, num.z += f * v[u].z, num.w += f * v[u].w;
-            }
+        for (int u = 0; u < 8; u++) {
+            const PartHead* p = reinterpret_cast<const PartHead*>(parts + min(s0 + u, A.splits - 1) * bytes);
+            ml[u] = s0 + u < A.splits ? __ldcg(&p->ml[r]) : make_float2(-INFINITY, 0.0f);
+            v[u] = s0 + u < A.splits && lane * 4 < pitch
+                       ? __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p + 1) + r * pitch + lane * 4))
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
-        const int i = r / at.heads, h = r - i * at.heads;
-        float* out = A.ctx + (static_cast<long>(at.b) * A.Rq + at.i0 + i) * A.ldc + static_cast<long>(at.head0 + h) * A.dv;
-        const float z[4] = {num.x * inv, num.y * inv, num.z * inv, num.w * inv};
+        float top = m;
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (lane * 4 + e < A.dv) out[lane * 4 + e] = z[e];
+        for (int u = 0; u < 8; u++) top = fmaxf(top, ml[u].x);
+        const float safe = top == -INFINITY ? 0.0f : top, back = kx::ex2_approx(m - safe);
+        m = top;
+        den *= back;
+        num.x *= back, num.y *= back, num.z *= back, num.w *= back;
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            if (ml[u].x == -INFINITY) continue;  // that part saw nothing of the row: its output may not be there
+            const float f = kx::ex2_approx(ml[u].x - safe);
+            den += f * ml[u].y;
+            num.x += f * v[u].x, num.y += f * v[u].y, num.z += f * v[u].z, num.w += f * v[u].w;
+        }
     }
+    // nothing to join (then the parts hold nothing, and what came of them is dropped), or behind the last row
+    if (!wanted || !lens_ok || r >= min(A.qt, ql - at.i0) * at.heads) return;
+    const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+    const int i = r / at.heads, h = r - i * at.heads;
+    float* out = A.ctx + (static_cast<long>(at.b) * A.Rq + at.i0 + i) * A.ldc + static_cast<long>(at.head0 + h) * A.dv;
+    const float z[4] = {num.x * inv, num.y * inv, num.z * inv, num.w * inv};
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (lane * 4 + e < A.dv) out[lane * 4 + e] = z[e];
 }
 
 struct WinLayout {
@@ -834,7 +846,7 @@ int kx_attention_window(const float* q, int ldq, const float* k, int ldk, const 
     const bool small = dk <= 64 && dv <= 64;
     if (A.splits == 1) return small ? launch_main<64, false>(A, grid, st) : launch_main<128, false>(A, grid, st);
     if ((small ? launch_main<64, true>(A, grid * A.splits, st) : launch_main<128, true>(A, grid * A.splits, st)) != 0) return -1;
-    return kx::launch_pdl(k_win_join, dim3(static_cast<unsigned>(grid) * 4), dim3(256), 0, st, A);
+    return kx::launch_pdl(k_win_join, dim3(static_cast<unsigned>(grid) * (WN_ROWS / 8)), dim3(256), 0, st, A);
 }
 
 }  // extern "C"
