@@ -27,9 +27,9 @@
 //    window of 2048: 771 us, 335 TFLOP/s of fp32 products; three fp16 products at the measured matrix rate are 461 us.
 //    One issuing thread for both products stood in its own way with heads of 64, whose products are short (a matrix
 //    instruction takes about 45 cycles to issue): 124 us against 111.
-//  Values that the parts cannot hold (NaN, infinities, magnitudes from 2^40 on) are flagged per tile by k_win_prep; a CTA
-//  that would read a flagged tile, or has such a q, computes its rows with plain fp32 code that reads only what each
-//  row sees.
+//  Tiles that the parts cannot hold (NaN, infinities, magnitudes from 2^40 on; a key or value row whose largest element is
+//  below 2^-14 of the tile's) are flagged by k_win_prep; a CTA that would read a flagged tile, or has such a q, computes
+//  its rows with plain fp32 code that reads only what each row sees.
 // Every wait is bounded; a timeout records KX_STATUS_TIMEOUT in the status word and the CTA stops.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -55,6 +55,7 @@ constexpr int WN_THREADS = 3 * WN_GROUP;
 // which two threads fetch and issue, keeps 40: 256 x 232 + 128 x 40 = 64,512
 constexpr int WN_DMAX = 128;
 constexpr float WN_HUGE = 1099511627776.0f;  // 2^40
+constexpr float WN_RANGE = 16384.0f;         // 2^14: the rows of a tile keep 2^-24 of their own largest value
 
 struct WinArgs {
     const float *q, *k, *v;
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(256) k_win_prep(const __grid_constant__ WinArg
         if (tile >= t.na && tile < t.b0) return;
     }
     bool good = true;
-    float ktop = 0.0f, vtop = 0.0f;
+    float ktop = 0.0f, vtop = 0.0f, krow[WN_KEYS / 8], vrow[WN_KEYS / 8];
     const float* kr = A.k + (static_cast<long>(b) * A.S + j0) * A.ldk + h * A.dk;
     const float* vr = A.v + (static_cast<long>(b) * A.S + j0) * A.ldv + h * A.dv;
     // a warp per row, all of its rows asked for at once; rows behind the last key are zero
@@ -197,27 +198,38 @@ __global__ void __launch_bounds__(256) k_win_prep(const __grid_constant__ WinArg
         const int r = warp + 8 * u;
         const float4 x = kx4[u], y = vx4[u];
         good = good && held4(x) && held4(y);
-        ktop = top4(ktop, x);
-        vtop = top4(vtop, y);
+        krow[u] = top4(0.0f, x);
+        vrow[u] = top4(0.0f, y);
         float *kd = ks + r * P + lane * 4, *vd = vs + r * P + lane * 4;
         kd[0] = x.x, kd[1] = x.y, kd[2] = x.z, kd[3] = x.w;
         vd[0] = y.x, vd[1] = y.y, vd[2] = y.z, vd[3] = y.w;
     }
+    // the rows' largest magnitudes, then the tile's
 #pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        ktop = fmaxf(ktop, __shfl_xor_sync(FULL, ktop, d));
-        vtop = fmaxf(vtop, __shfl_xor_sync(FULL, vtop, d));
+    for (int u = 0; u < WN_KEYS / 8; u++) {
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            krow[u] = fmaxf(krow[u], __shfl_xor_sync(FULL, krow[u], d));
+            vrow[u] = fmaxf(vrow[u], __shfl_xor_sync(FULL, vrow[u], d));
+        }
+        ktop = fmaxf(ktop, krow[u]);
+        vtop = fmaxf(vtop, vrow[u]);
     }
     if (lane == 0) {
         tops[0][warp] = ktop;
         tops[1][warp] = vtop;
     }
-    good = __syncthreads_and(good);
+    __syncthreads();
 #pragma unroll
     for (int w = 0; w < 8; w++) {
         ktop = fmaxf(ktop, tops[0][w]);
         vtop = fmaxf(vtop, tops[1][w]);
     }
+    // a row far below the tile's largest would lose bits to its neighbour, which its query may not even see
+#pragma unroll
+    for (int u = 0; u < WN_KEYS / 8; u++)
+        good = good && (krow[u] == 0.0f || krow[u] * WN_RANGE >= ktop) && (vrow[u] == 0.0f || vrow[u] * WN_RANGE >= vtop);
+    good = __syncthreads_and(good);
     float kdown, vdown;
     const float kup = scale_up(ktop, -100, &kdown), vup = scale_up(vtop, -40, &vdown);
     uint8_t* out = A.ws + static_cast<size_t>(blockIdx.x) * A.block;

@@ -247,6 +247,39 @@ def test_values_that_parts_cannot_hold(kx, what):
         assert float((ctx[i, h].cpu().double() - p @ v[0, :, h // 2]).abs().max()) <= 2.0**-17 * float(v.abs().max())
 
 
+@pytest.mark.parametrize("far", [1e6, 3e8, 1e11, -1e9])
+@pytest.mark.parametrize("what", ["k", "v", "both"])
+def test_one_row_far_above_its_neighbours(kx, what, far):
+    """finite, but so far above the rest of its tile that common scales would cost the others their bits: rows that do not see
+    it are as exact as ever, rows that do follow the formula, whether it takes all of the weight or none"""
+    def make(value):
+        c = Case(1, 300, 300, 4, 2, 64, 64, window=120, sinks=2, seed=3)
+        if what != "v":
+            c.k[0, 100, 0, 9] = value
+        if what != "k":
+            c.v[0, 100, 0, 7] = value
+        return c
+    c, clean = make(far), make(1.0)
+    got, want = c.run(kx).view(300, 4, 64).clone(), clean.run(kx).view(300, 4, 64)
+    top = float(clean.v.abs().max())
+    unseen = torch.ones(300, 4, dtype=torch.bool)
+    unseen[100:220, :2] = False
+    unseen = unseen.cuda()
+    assert float((got - want)[unseen].abs().max()) <= 2.0**-17 * top
+    q, k, v = (x.double().cuda() for x in (c.q, c.k, c.v))
+    seen = c.seen(0).cuda()
+    for h in range(2):
+        s = (q[0, :, h] @ torch.where(torch.isfinite(k[0, :, 0]), k[0, :, 0], 0.0).T / 8).masked_fill(~seen, -math.inf)
+        p = torch.softmax(s, 1)
+        v0 = torch.where(torch.isfinite(v[0, :, 0]), v[0, :, 0], 0.0)
+        # against the weights' share of the far value, and of the others
+        tol = 2.0**-15 * (p @ v0.abs())[100:220] + 2.0**-17 * top
+        err = (got[100:220, h].double() - (p @ v0)[100:220]).abs()
+        if what != "v":  # scores of 1e6 and more are only good to 2^-24 of themselves in fp32: rows where two keys tie are left out
+            err, tol = err[(s[100:220].topk(2).values.diff(dim=1).abs() > 1).squeeze(1)], tol[(s[100:220].topk(2).values.diff(dim=1).abs() > 1).squeeze(1)]
+        assert bool((err <= tol).all()), float((err / tol).max())
+
+
 def test_bad_lengths(kx):
     for ql, kl in (([5, -1], [9, 9]), ([11, 3], [9, 9]), ([5, 5], [10, 9]), ([5, 5], [9, -2])):
         c = Case(2, 10, 9, 2, 1, 32, 32, q_len=[5, 5], k_len=[9, 9])
