@@ -24,7 +24,7 @@
 //    Bound: the chain S -> softmax -> P.V of a group and, close to it, the tensor cores (for heads of 128 a tile's
 //    products are 1536 cycles of tensor work; measured 2240 per tile, in which each group's softmax is 1500 of its 4480)
 //    plus a CTA's beginning and end, one fifth of its time. 16384 rows of 16 heads of 128 over 4 key-value heads with a
-//    window of 2048: 771 us, 335 TFLOP/s of fp32 products; three fp16 products at the measured matrix rate are 461 us.
+//    window of 2048: 749 us, 345 TFLOP/s of fp32 products; three fp16 products at the measured matrix rate are 461 us.
 //    One issuing thread for both products stood in its own way with heads of 64, whose products are short (a matrix
 //    instruction takes about 45 cycles to issue): 124 us against 111.
 //  Tiles that the parts cannot hold (NaN, infinities, magnitudes from 2^40 on; a key or value row whose largest element is
