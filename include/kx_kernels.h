@@ -257,7 +257,8 @@ KERNIX_API int kx_attention(const float* q, int ldq, const float* k, int ldk, co
  * An empty cache has lens = 0, refs = 0, table = -1; the entry points below keep these consistent.
  * Requirements, else -1: page a power of two up to 1024; dk * size and dv * size multiples of 16 bytes, dk, dv <= 1024;
  * k, v and all strides * size multiples of 16 bytes; pages (and layers) that do not overlap;
- * max_pages * page < 2^31; heads * page * dk and heads * page * dv <= 2^28. Calls that change a cache are ordered on one stream (or by events) with those that use it.
+ * max_pages * page < 2^31; heads * page * dk and heads * page * dv <= 2^28. Calls that change a cache are ordered on one
+ * stream (or by events) with those that use it.
  *
  * Requests live in device memory, so a kernel checks them: what it refuses it leaves out, memory-safely, and ORs a bit
  * into *status (device word, may be NULL; never cleared here): KX_STATUS_NO_PAGES, too few free pages or a full table
@@ -320,9 +321,9 @@ KERNIX_API int kx_kv_compact(const kx_kv* c, int32_t* n_live, void* ws, size_t w
  * when window <= 0, or j > lens - 1 - window, or j < sinks. ctx + i * ldc receives H * dv floats. scale 0 means
  * 1/sqrt(dk). A row with seqs[i] < 0 is left as it was, one whose slot holds no tokens becomes 0, and one whose slot,
  * length or (visible) pages are out of range becomes NaN and is reported. Keys and values that are not seen do not affect
- * results, whatever they hold; those that are have to be finite and, in an fp32 cache, below 2^127 (a head that sees an infinite key becomes NaN, a column
- * with an infinite value NaN). H a multiple of heads, dk, dv <= 128. q and ctx
- * must not overlap each other or the cache. ws: kx_attention_paged_ws bytes of device workspace (0: the arguments are
+ * results, whatever they hold; those that are have to be finite and, in an fp32 cache, below 2^127 (a head that sees an
+ * infinite key becomes NaN, a column with an infinite value NaN). H a multiple of heads, dk, dv <= 128. q and ctx must not
+ * overlap each other or the cache. ws: kx_attention_paged_ws bytes of device workspace (0: the arguments are
  * invalid), to be shared under kx_kv_ws's rules. Results do not depend on timing: the same call on the same contents
  * gives the same bits. */
 KERNIX_API size_t kx_attention_paged_ws(const kx_kv* c, int H, int n);
@@ -341,8 +342,9 @@ KERNIX_API int kx_attention_paged(const kx_kv* c, int layer, const float* q, int
  * of device workspace (0: the arguments are invalid), 128-byte aligned, shared under kx_kv_ws's rules. Key and value
  * rows that no query of the sample sees do not affect results, whatever they hold. Accuracy is fp32's: products keep 2^-22
  * of their operands, where an element of q (k or v) is not below 2^-16 of the largest in its row (in its 64 rows); below
- * that they keep 2^-38 of that largest. Blocks of 128 rows that see NaN, infinities, magnitudes of 2^40 and more, or rows of
- * k or v 2^14 times above one of their neighbours, are computed by plain fp32 code, at a small fraction of the speed. */
+ * that they keep 2^-38 of that largest. Blocks of 128 rows that see NaN, infinities, magnitudes of 2^40 and more, rows of
+ * k or v 2^14 times above one of their neighbours, or 64 rows of v all below 2^-40, are computed by plain fp32 code, at a
+ * small fraction of the speed. */
 KERNIX_API size_t kx_attention_window_ws(int B, int S, int Hkv, int dk, int dv);
 KERNIX_API int kx_attention_window(const float* q, int ldq, const float* k, int ldk, const float* v, int ldv, float* ctx, int ldc,
                                    int B, int Rq, int S, int H, int Hkv, int dk, int dv, const int32_t* q_len, const int32_t* k_len,

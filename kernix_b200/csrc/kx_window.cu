@@ -28,7 +28,7 @@
 //    One issuing thread for both products stood in its own way with heads of 64, whose products are short (a matrix
 //    instruction takes about 45 cycles to issue): 124 us against 111.
 //  Tiles that the parts cannot hold (NaN, infinities, magnitudes from 2^40 on; a key or value row whose largest element is
-//  below 2^-14 of the tile's) are flagged by k_win_prep; a CTA that would read a flagged tile, or has such a q, computes
+//  below 2^-14 of the tile's; nothing but values below 2^-40) are flagged by k_win_prep; a CTA that would read a flagged tile, or has such a q, computes
 //  its rows with plain fp32 code that reads only what each row sees.
 // Every wait is bounded; a timeout records KX_STATUS_TIMEOUT in the status word and the CTA stops.
 #include <cuda_fp16.h>
@@ -55,6 +55,10 @@ constexpr int WN_THREADS = 3 * WN_GROUP;
 // which two threads fetch and issue, keeps 40: 256 x 232 + 128 x 40 = 64,512
 constexpr int WN_DMAX = 128;
 constexpr float WN_HUGE = 1099511627776.0f;  // 2^40
+// value tiles' scales go no lower: an output in the units of a tile of 2^40 is shrunk by 2^-80, one of the lowest
+// tile grows by 2^80 from at most 2^33, both inside fp32's range
+constexpr int WN_LOW = -40;
+constexpr float WN_TINY = 9.094947e-13f;     // 2^-40
 constexpr float WN_RANGE = 16384.0f;         // 2^14: the rows of a tile keep 2^-24 of their own largest value
 
 struct WinArgs {
@@ -140,7 +144,8 @@ __device__ __forceinline__ void parts2(float a, float b, uint32_t* hi, uint32_t*
     *lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 // the power of two that brings `top` (the largest magnitude) into [2^13, 2^14), and its inverse
-// (top < 2^40; what is below 2^lowest keeps its distance to that)
+// (top < 2^40; what is below 2^lowest keeps its distance to that: scores of q or keys below 2^-100 are as good as zero, and
+// value tiles below 2^WN_LOW go the plain way)
 __device__ __forceinline__ float scale_up(float top, int lowest, float* down) {
     const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23) - 127, lowest), 40);
     *down = __uint_as_float(static_cast<uint32_t>(127 - 13 + e) << 23);
@@ -229,9 +234,10 @@ __global__ void __launch_bounds__(256) k_win_prep(const __grid_constant__ WinArg
 #pragma unroll
     for (int u = 0; u < WN_KEYS / 8; u++)
         good = good && (krow[u] == 0.0f || krow[u] * WN_RANGE >= ktop) && (vrow[u] == 0.0f || vrow[u] * WN_RANGE >= vtop);
+    good = good && (vtop == 0.0f || vtop >= WN_TINY);
     good = __syncthreads_and(good);
     float kdown, vdown;
-    const float kup = scale_up(ktop, -100, &kdown), vup = scale_up(vtop, -40, &vdown);
+    const float kup = scale_up(ktop, -100, &kdown), vup = scale_up(vtop, WN_LOW, &vdown);
     uint8_t* out = A.ws + static_cast<size_t>(blockIdx.x) * A.block;
     // K: chunk c of 8 head dims of key r; eight threads write a plane's row
     for (int x = tid; x < WN_KEYS * 8 * A.ka; x += 256) {

@@ -192,6 +192,16 @@ def test_small_and_large_values(kx, big):
     c.check(c.run(kx))
 
 
+@pytest.mark.parametrize("big", [1e-8, 1e-13, 1e-20, 1e-32, 1e10, 1e15])
+@pytest.mark.parametrize("Rq", [9, 300])
+def test_small_and_large_v(kx, big, Rq):
+    """outputs as exact relative to their own values, whatever their size"""
+    c = Case(2, Rq, 300, 4, 2, 64, 80, window=90, sinks=3, seed=12)
+    c.v *= big
+    c.check(c.run(kx))
+    assert int(c.status) == 0
+
+
 def test_one_large_value_among_small_ones(kx):
     """a key and a value 2^12 times the others in their tile: the others keep their accuracy"""
     c = Case(1, 200, 200, 2, 2, 64, 64)
