@@ -60,6 +60,10 @@ constexpr float WN_HUGE = 1099511627776.0f;  // 2^40
 constexpr int WN_LOW = -40;
 constexpr float WN_TINY = 9.094947e-13f;     // 2^-40
 constexpr float WN_RANGE = 16384.0f;         // 2^14: the rows of a tile keep 2^-24 of their own largest value
+// Scores (in base 2) from here on are rounded before the maximum is taken off, as the maximum is: the unrounded product
+// less the rounded maximum is off by half a unit of the score, which for scores of 2^25 and more carries p out of fp16's
+// range either way (NaN, or rows of zeros). Below, it is off by 2^-4 at most.
+constexpr float WN_FAR = 1048576.0f;         // 2^20
 
 struct WinArgs {
     const float *q, *k, *v;
@@ -626,7 +630,9 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                     for (int y = 0; y < 32; y++) top[y & 3] = fmaxf(top[y & 3], __uint_as_float(x[y]));
                 }
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                const float mn = mx == -INFINITY ? m : fmaxf(m, mx * f), safe = mn == -INFINITY ? 0.0f : mn, shift = 13.0f - safe;
+                const float mn = mx == -INFINITY ? m : fmaxf(m, __fmul_rn(mx, f)), safe = mn == -INFINITY ? 0.0f : mn;
+                const bool far = __any_sync(FULL, fabsf(safe) >= WN_FAR);
+                const float mul = far ? 1.0f : f, shift = far ? 13.0f : 13.0f - safe;
                 alpha = kx::ex2_approx(m - safe);
                 m = mn;
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
@@ -634,10 +640,14 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                 for (int c = 0; c < 2; c++) {
                     uint32_t(&x)[32] = s[D > 64 ? 0 : c];
                     if (D > 64) load(c, x);
+                    if (far) {
+#pragma unroll
+                        for (int y = 0; y < 32; y++) x[y] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(x[y]), f), -safe));
+                    }
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int y = 0; y < 32; y += 2) {
-                        float2 e = kx::fma2(make_float2(__uint_as_float(x[y]), __uint_as_float(x[y + 1])), make_float2(f, f),
+                        float2 e = kx::fma2(make_float2(__uint_as_float(x[y]), __uint_as_float(x[y + 1])), make_float2(mul, mul),
                                             make_float2(shift, shift));
                         e.x = kx::ex2_approx(e.x);
                         e.y = kx::ex2_approx(e.y);
