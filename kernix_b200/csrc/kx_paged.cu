@@ -404,7 +404,8 @@ struct Tile {
             }
 #pragma unroll
             for (int e = 0; e < 2; e++)
-                s[2 * u + e] = ((dd[0][e] + dd[1][e]) + ((dd[0][e + 2] + dd[1][e + 2]) + (dd[2][e] + dd[3][e]))) * qscale;
+                // rounded here for good: a product that reached the exponential unrounded would pass its own maximum
+                s[2 * u + e] = __fmul_rn((dd[0][e] + dd[1][e]) + ((dd[0][e + 2] + dd[1][e + 2]) + (dd[2][e] + dd[3][e])), qscale);
             if (FEW) {
 #pragma unroll
                 for (int e = 0; e < 2; e++) s[2 * u + e] += __shfl_xor_sync(FULL, s[2 * u + e], 16);
@@ -433,7 +434,7 @@ struct Tile {
         float p[2 * S::KT];
 #pragma unroll
         for (int e = 0; e < 2 * S::KT; e++) {
-            p[e] = kx::ex2_approx(s[e] - (safe - off));
+            p[e] = kx::ex2_approx((s[e] - safe) + off);  // the maximum's is 2^off, however large the scores are
             l += p[e];
         }
         // p.v: column 2 t (2 t + 1) of n-tile (k, e) is element e of chunk 8 k + t (+ 4); row t + 4 x of the step is x-th

@@ -62,3 +62,54 @@ def test_large_scores_of_one_sign(kx, sign, score):  # noqa: F811
     c.q[0, :, :, :4] = sign * score / 4 / 2.0**8 * math.sqrt(32)
     assert one_hot_rows(c, c.run(kx)) == 2 * 200
     assert int(c.status) == 0
+
+
+def scored(dtype, scores, v, heads=1, group=2, page=16, q0=1.0):
+    """A cache (test_gpu_paged.Case) of rows whose keys have the given scores: key j is scores[j] / (4 q0) four times, q is
+    q0 four times, the scale 1. scores: (rows, keys), v: (rows, keys, dv)."""
+    import test_gpu_paged as tp
+    rows, keys = scores.shape
+    c = tp.Case([keys] * rows, heads, group, 64, v.shape[2], page, dtype)
+    c.host = []
+    k = torch.zeros(rows, keys, heads, 64, dtype=torch.float64)
+    k[..., :4] = (scores.double() / (4 * q0))[:, :, None, None]
+    stored = k.to(tp.DTYPES[dtype])
+    assert bool((stored.double() == k).all())  # the scores are what was asked for
+    values = v[:, :, None].expand(-1, -1, heads, -1).to(tp.DTYPES[dtype])
+    j = torch.arange(keys)
+    for r in range(rows):
+        p = c.table[r, j.cuda() // page].long()
+        c.k[0][p, :, j.cuda() % page] = stored[r].cuda()
+        c.v[0][p, :, j.cuda() % page] = values[r].cuda()
+        c.host.append((stored[r].double().numpy(), values[r].double().numpy()))
+    c.q = torch.zeros(rows, heads * group, 64)
+    c.q[..., :4] = q0
+    c.q = c.q.view(rows, -1)
+    return c
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("keys", [90, 4000])
+def test_large_scores_over_the_cache(kx, dtype, sign, keys):  # noqa: F811
+    """The largest base-2 scores from 2^18 to 2^40, by both launches: one key leads by 1/8 of its score, every other weight is 0;
+    the value keeps 2^-18 (its weight's parts and the division)."""
+    tops = [2.0**18, 2.0**24, 2.0**25, 1.25 * 2.0**25, 2.0**26, 1.25 * 2.0**26, 1.5 * 2.0**26, 2.0**27, 1.75 * 2.0**27, 2.0**28, 2.0**40]
+    g = torch.Generator().manual_seed(keys)
+    near = torch.randint(5, 8, (len(tops), keys), generator=g).double()  # eighths; negative scores: the least of them leads
+    lead = torch.randint(0, keys, (len(tops),), generator=g)
+    near[torch.arange(len(tops)), lead] = 8 if sign > 0 else 4
+    scores = sign * near / 8 * torch.tensor(tops, dtype=torch.float64)[:, None]
+    v = torch.randn(len(tops), keys, 72, generator=g)
+    if sign < 0:
+        scores *= 2
+    # the keys' part of a score is below 2^12, so that every cache holds it; q takes the rest
+    got = []
+    for r, top in enumerate(tops):
+        q0 = top / 2.0**12
+        c = scored(dtype, scores[r:r + 1], v[r:r + 1], q0=q0)
+        got.append(c.run(kx, scale=1 / math.log2(math.e)).view(2, 72).cpu().double())
+        want = torch.from_numpy(c.host[0][1][lead[r], 0])
+        assert bool(got[-1].isfinite().all()), top
+        assert float((got[-1] - want).abs().max()) <= 2.0**-18 * float(v.abs().max()), top
+        assert int(c.status) == 0
