@@ -191,13 +191,15 @@ __global__ void __launch_bounds__(256) k_win_prep(const __grid_constant__ WinArg
     float ktop = 0.0f, vtop = 0.0f, krow[WN_KEYS / 8], vrow[WN_KEYS / 8];
     const float* kr = A.k + (static_cast<long>(b) * A.S + j0) * A.ldk + h * A.dk;
     const float* vr = A.v + (static_cast<long>(b) * A.S + j0) * A.ldv + h * A.dv;
-    // a warp per row, all of its rows asked for at once; rows behind the last key are zero
+    // a warp per row, all of its rows asked for at once; rows behind the last key and rows that no query sees (behind the
+    // first tokens, before the first query's window) are zero, so that they touch neither the scales nor the flag
+    const int back = kl - ql - A.window;  // the last position before every window
     float4 kx4[WN_KEYS / 8], vx4[WN_KEYS / 8];
 #pragma unroll
     for (int u = 0; u < WN_KEYS / 8; u++) {
         const int r = warp + 8 * u;
         kx4[u] = vx4[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < n) {
+        if (r < n && (A.window <= 0 || j0 + r > back || j0 + r < A.sinks)) {
             kx4[u] = load4(kr + static_cast<long>(r) * A.ldk, lane * 4, A.dk, A.veck);
             vx4[u] = load4(vr + static_cast<long>(r) * A.ldv, lane * 4, A.dv, A.vecv);
         }

@@ -113,3 +113,25 @@ def test_large_scores_over_the_cache(kx, dtype, sign, keys):  # noqa: F811
         assert bool(got[-1].isfinite().all()), top
         assert float((got[-1] - want).abs().max()) <= 2.0**-18 * float(v.abs().max()), top
         assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("Rq,S,window,sinks,dk", [(150, 700, 100, 5, 64), (150, 700, 90, 0, 128), (9, 3000, 1500, 70, 64),
+                                                   (20, 2500, 1111, 3, 128), (64, 70, 3, 2, 32)])
+def test_unseen_rows_leave_no_trace(kx, Rq, S, window, sinks, dk):  # noqa: F811
+    """the same bits whatever lies in rows that no query sees, behind the last key or in the rows behind the queries"""
+    k_len, q_len = [S, S - 30, S], [Rq, Rq - 3, 1]
+    out = []
+    for fill in (0.0, float("nan"), float("inf"), 1e6, 1e-30, -3e38):
+        c = Case(3, Rq, S, 4, 2, dk, 64, window, sinks, q_len=q_len, k_len=k_len, seed=6)
+        for b in range(3):
+            unseen = torch.ones(S, dtype=torch.bool)
+            unseen[: k_len[b]] = ~c.seen(b).any(0)
+            assert b or bool(unseen.any())
+            c.k[b][unseen] = fill
+            c.v[b][unseen] = fill
+            c.q[b, q_len[b]:] = fill
+        out.append(c.run(kx).clone())
+        assert int(c.status) == 0
+    c.check(out[0])
+    for o in out[1:]:
+        assert torch.equal(o, out[0])
