@@ -341,8 +341,8 @@ KERNIX_API int kx_attention_paged(const kx_kv* c, int layer, const float* q, int
  * 1/sqrt(dk). dk, dv <= 128, H a multiple of Hkv. q, k, v must not overlap ctx or ws. ws: kx_attention_window_ws bytes
  * of device workspace (0: the arguments are invalid), 128-byte aligned, shared under kx_kv_ws's rules. Key and value
  * rows that no query of the sample sees do not affect results, whatever they hold. Accuracy is fp32's: products keep 2^-22
- * of their operands, where an element of q (k or v) is not below 2^-16 of the largest in its row (in its 64 rows); below
- * that they keep 2^-38 of that largest. Blocks of 128 rows that see NaN, infinities, magnitudes of 2^40 and more, rows of
+ * of their operands, where an element of q (k or v) is not below 2^-16 of the largest in its row (in its 64 rows), or a
+ * weight not below 2^-16 of the largest that its row has among those 64 keys; below that they keep 2^-38 of that largest. Blocks of 128 rows that see NaN, infinities, magnitudes of 2^40 and more, rows of
  * k or v 2^14 times above one of their neighbours, or 64 rows of v all below 2^-40, are computed by plain fp32 code, at a
  * small fraction of the speed. */
 KERNIX_API size_t kx_attention_window_ws(int B, int S, int Hkv, int dk, int dv);

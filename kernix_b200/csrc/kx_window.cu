@@ -6,8 +6,10 @@
 // 64 keys) is in [2^13, 2^14), is the sum of two fp16 parts up to 2^-22 of itself (up to 2^-39 of that largest where
 // that is more), and a.b = ah.bh + al.bh + ah.bl: three fp16 products where 3xTF32 (the same 11-bit parts, no scaling)
 // would cost six fp16 products' time. One scale per query row and one per tile of keys and of values: they are undone
-// in fp32, the scores' in the exponential's multiply-add, the values' by keeping the output in the units of the latest
-// tile (a ratio of two powers of two joins the factor by which a new maximum shrinks it). p in [0, 1] becomes p 2^13.
+// in fp32, the scores' in the exponential's multiply-add, the values' by the factor with which a tile's P.V joins the
+// output. p is taken relative to the row's largest score in the tile, not to its running maximum, and becomes p 2^13: it
+// keeps 2^-22 of itself, or 2^-38 of that largest where that is more, whatever other tiles hold (relative to the running
+// maximum, small weights of a tile of much larger values lost the bits that their products needed).
 // (A scale per key and per value column of a tile cost as many instructions as the rest of the softmax together:
 // 237 us against 224 for 4096 rows of 16 heads of 128 with a window of 2048, before the steps that made it 179.)
 //
@@ -55,9 +57,12 @@ constexpr int WN_THREADS = 3 * WN_GROUP;
 // which two threads fetch and issue, keeps 40: 256 x 232 + 128 x 40 = 64,512
 constexpr int WN_DMAX = 128;
 constexpr float WN_HUGE = 1099511627776.0f;  // 2^40
-// value tiles' scales go no lower: an output in the units of a tile of 2^40 is shrunk by 2^-80, one of the lowest
-// tile grows by 2^80 from at most 2^33, both inside fp32's range
+// value tiles' scales go no lower, so that the factor of P.V (the scale, 2^-53 at least, times a tile's share) is a normal
+// number for every share that can show next to others
 constexpr int WN_LOW = -40;
+// A row's output and sum are relative to a score that its largest may pass by this (in base 2) before they are scaled to
+// it: fp32 has the room, and tiles that scale nothing save a pass over the output.
+constexpr float WN_SLACK = 16.0f;
 constexpr float WN_TINY = 9.094947e-13f;     // 2^-40
 constexpr float WN_RANGE = 16384.0f;         // 2^14: the rows of a tile keep 2^-24 of their own largest value
 // Scores (in base 2) from here on are rounded before the maximum is taken off, as the maximum is: the unrounded product
@@ -286,7 +291,7 @@ struct Win {
     static constexpr uint32_t TQH = 0, TQL = D / 2, TS = D, TO = 256, COLS = 512;
     static_assert(TS + NS * WN_KEYS <= TO && TO + 2 * D <= COLS, "tensor memory");
     static_assert(K2 + WN_ROWS * D * 4 <= TOPS, "q's rows fit");
-    static_assert(TOPS >= WN_ROWS * (D + 2 + 6) * 4, "the groups' halves, maxima, sums and units fit in the tiles' place");
+    static_assert(TOPS >= WN_ROWS * (D + 2 + 4) * 4, "the groups' halves, maxima and sums fit in the tiles' place");
     __device__ __forceinline__ static int k_at(int s) { return s < 2 ? s * KB : K2; }
     __device__ __forceinline__ static int v_at(int s) { return s < 2 ? V0 + s * VB : V2; }
 };
@@ -573,15 +578,15 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
         __syncwarp();
     } else {  // softmax groups
         asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
-        float2 o[D / 2];  // times `unit`: the row's output so far
-        float m = -INFINITY, l = 0.0f, unit = 1.0f;
+        float2 o[D / 2];  // the row's output so far and its sum l, relative to a score of m
+        float m = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int y = 0; y < D / 2; y++) o[y] = make_float2(0.0f, 0.0f);
         const uint32_t om = tmem + lanes + W::TO + grp * D;
         const int p_first = off + i0, p_last = off + i0 + nq - 1;
         float2 scales = make_float2(1.0f, 1.0f);  // a tile's, fetched a tile ahead
         if (grp < n) scales = __ldcg(reinterpret_cast<const float2*>(info + tile_at(grp)));
-        float keep = 1.0f, keep_next = 1.0f;
+        float gain = 0.0f, gain_next = 0.0f;  // what P.V is multiplied with: its tile's scale and share
         const auto join = [&](int t) {  // P.V of tile t joins the output
             if (!__all_sync(FULL, kx::mbar_wait(&ctl.ofull[grp], (t / 2) & 1, &ctl.abort, A.status))) return false;
             kx::tc_fence_after();
@@ -593,23 +598,23 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                 kx::tmem_ld32_wait(d);
 #pragma unroll
                 for (int y = 0; y < 32; y += 2)
-                    o[(c + y) / 2] = kx::fma2(o[(c + y) / 2], make_float2(keep, keep),
-                                              make_float2(__uint_as_float(d[y]), __uint_as_float(d[y + 1])));
+                    o[(c + y) / 2] = kx::fma2(make_float2(__uint_as_float(d[y]), __uint_as_float(d[y + 1])), make_float2(gain, gain),
+                                              o[(c + y) / 2]);
             }
             kx::tc_fence_before();
             return true;
         };
         for (int t = grp; grp < n; t += 2) {
+            float alpha = 1.0f;
+            bool moved = false;  // m grows: what there is of the output shrinks by alpha
             if (t < n) {  // P of tile t
                 const uint32_t sm = tmem + lanes + W::TS + (t % W::NS) * WN_KEYS;
                 const int j0 = tile_at(t) * WN_KEYS;
                 const float f = fmaxf(cs * scales.x, 1.17549435e-38f);  // positive: -inf stays -inf
-                const float shrink = unit * (1.0f / scales.y);           // powers of two
-                unit = scales.y;
+                const float vscale = scales.y;
                 if (t + 2 < n) scales = __ldcg(reinterpret_cast<const float2*>(info + tile_at(t + 2)));
                 if (!__all_sync(FULL, kx::mbar_wait(&ctl.sfull[t % W::NS], (t / W::NS) & 1, &ctl.abort, A.status))) break;
                 kx::tc_fence_after();
-                float alpha;
                 // some row does not see some key of the tile
                 const bool masked = j0 + WN_KEYS - 1 > p_first || !(A.window <= 0 || j0 > p_last - A.window || j0 + WN_KEYS <= A.sinks);
                 const int from = A.window > 0 ? my_p - A.window - j0 : -1, to = my_p - j0, first = A.sinks - j0;
@@ -632,11 +637,15 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                     for (int y = 0; y < 32; y++) top[y & 3] = fmaxf(top[y & 3], __uint_as_float(x[y]));
                 }
                 const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                const float mn = mx == -INFINITY ? m : fmaxf(m, __fmul_rn(mx, f)), safe = mn == -INFINITY ? 0.0f : mn;
+                const float peak = __fmul_rn(mx, f), safe = peak == -INFINITY ? 0.0f : peak;
+                if (peak > m + WN_SLACK) {
+                    moved = m != -INFINITY;
+                    alpha = kx::ex2_approx(m - peak);
+                    m = peak;
+                }
+                const float share = kx::ex2_approx(peak - (m == -INFINITY ? 0.0f : m));
                 const bool far = __any_sync(FULL, fabsf(safe) >= WN_FAR);
                 const float mul = far ? 1.0f : f, shift = far ? 13.0f : 13.0f - safe;
-                alpha = kx::ex2_approx(m - safe);
-                m = mn;
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
@@ -659,12 +668,16 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                     kx::tmem_st16(sm + c * 32, hi);
                     kx::tmem_st16(sm + c * 32 + 16, lo);
                 }
-                l = l * alpha + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
-                keep_next = alpha * shrink;
+                l = l * alpha + share * ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+                gain_next = share * vscale;
             }
             if (W::AHEAD && t >= 2 && !join(t - 2)) break;
             if (t >= n) break;
-            keep = keep_next;
+            if (__any_sync(FULL, moved)) {
+#pragma unroll
+                for (int y = 0; y < D / 2; y++) o[y] = kx::mul2(o[y], make_float2(alpha, alpha));
+            }
+            gain = gain_next;
             kx::tmem_st_wait();
             kx::tc_fence_before();
             kx::mbar_arrive(&ctl.pready[grp]);
@@ -675,10 +688,10 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
         if (n > 0) {
             constexpr int P = D / 2 + 1;
             float* half = reinterpret_cast<float*>(smem);  // [group that joins it][row][column]
-            float* ml = half + 2 * WN_ROWS * P;            // [group][row]: maximum, sum and unit
+            float* ml = half + 2 * WN_ROWS * P;            // [group][row]: what it is relative to, and the sum
             kx::named_bar(3, 2 * WN_GROUP);
-            float* mine = ml + (grp * WN_ROWS + r) * 3;
-            mine[0] = m, mine[1] = l, mine[2] = unit;
+            float* mine = ml + (grp * WN_ROWS + r) * 2;
+            mine[0] = m, mine[1] = l;
             float* send = half + ((grp ^ 1) * WN_ROWS + r) * P;
 #pragma unroll
             for (int x = 0; x < D / 4; x++) {
@@ -687,13 +700,13 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
             }
             kx::named_bar(3, 2 * WN_GROUP);
             {
-                const float* his = ml + ((grp ^ 1) * WN_ROWS + r) * 3;
+                const float* his = ml + ((grp ^ 1) * WN_ROWS + r) * 2;
                 const float mm = fmaxf(m, his[0]), safe = mm == -INFINITY ? 0.0f : mm;
                 float f0 = kx::ex2_approx(m - safe), f1 = kx::ex2_approx(his[0] - safe);
                 const float den = f0 * l + f1 * his[1];
                 if (SPLIT && grp == 0) part()->ml[r] = make_float2(mm, den);
                 const float inv = SPLIT ? 1.0f : den == 0.0f ? 0.0f : 1.0f / den;
-                f0 *= inv * unit, f1 *= inv * his[2];
+                f0 *= inv, f1 *= inv;
                 float* z = half + (grp * WN_ROWS + r) * P;
 #pragma unroll
                 for (int x = 0; x < D / 4; x++) {

@@ -135,3 +135,33 @@ def test_unseen_rows_leave_no_trace(kx, Rq, S, window, sinks, dk):  # noqa: F811
     c.check(out[0])
     for o in out[1:]:
         assert torch.equal(o, out[0])
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (32, 128)])
+@pytest.mark.parametrize("Rq,S", [(512, 512), (5, 2000)])
+@pytest.mark.parametrize("far,drop", [(2.0**18, -17.375), (2.0**25, -20.75), (2.0**30, -20.75), (2.0**38, -26.375), (2.0**39, -20)])
+def test_tiles_of_far_values_under_small_weights(kx, Rq, S, dk, dv, far, drop):  # noqa: F811
+    """Every other pair of 64-key tiles holds values `far` times the others' under weights of about e^drop: the output keeps
+    its bits relative to sum p|v|, whichever comes first. Scores are single exact products; the exponential's argument is
+    off by three roundings of at most 40 (2^-24 each) and a weight twice by that; p's and the values' parts, the
+    exponential and the sums: 2^-18, as everywhere."""
+    for first in (0, 1):
+        c = Case(1, Rq, S, 2, 1, dk, dv, seed=17)
+        j = torch.arange(S)
+        high = (j // 128) % 2 == first
+        g = torch.Generator().manual_seed(4)
+        score = torch.randint(-16, 1, (S,), generator=g) / 8 + torch.where(high, drop, 0.0)
+        c.k[:] = 0
+        c.k[0, :, 0, 1] = score
+        c.q[:] = 0
+        c.q[..., 1] = 1
+        c.v = c.v.sign() * (1 + torch.rand(c.v.shape, generator=g))
+        c.v[0, high] *= far
+        got = c.run(kx, scale=1.0).double().view(Rq, 2, dv)
+        seen, v = c.seen(0).cuda(), c.v[0, :, 0].double().cuda()
+        p = torch.exp(score.double().cuda())[None] * seen
+        p = p / p.sum(1, keepdim=True)
+        size = p @ v.abs().amax(1)
+        tol = math.expm1(2 * 3 * 40 * 2.0**-24) + 2.0**-18
+        assert float(((got - (p @ v)[:, None]).abs() / size[:, None, None]).max()) <= tol
+        assert int(c.status) == 0
