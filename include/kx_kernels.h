@@ -323,7 +323,9 @@ KERNIX_API int kx_kv_compact(const kx_kv* c, int32_t* n_live, void* ws, size_t w
  * length or (visible) pages are out of range becomes NaN and is reported. Keys and values that are not seen do not affect
  * results, whatever they hold; those that are have to be finite and, in an fp32 cache, below 2^127 (a head that sees an
  * infinite key becomes NaN, a column with an infinite value NaN). H a multiple of heads, dk, dv <= 128. q and ctx must not
- * overlap each other or the cache. ws: kx_attention_paged_ws bytes of device workspace (0: the arguments are
+ * overlap each other or the cache. Accuracy is fp32's; against an f16 cache q keeps 2^-22 of itself, or 2^-38 of its head's
+ * largest element where that is more, and a weight 2^-22 of itself or 2^-38 of the largest among its 16 keys (positions 16 i to
+ * 16 i + 15). ws: kx_attention_paged_ws bytes of device workspace (0: the arguments are
  * invalid), to be shared under kx_kv_ws's rules. Results do not depend on timing: the same call on the same contents
  * gives the same bits. */
 KERNIX_API size_t kx_attention_paged_ws(const kx_kv* c, int H, int n);

@@ -9,7 +9,8 @@
 //     CUDA cores no more than one would (plain multiplies in fp32 would be as long as the loads from 4 heads per
 //     key-value head on). The cache's elements enter exactly as they are stored; the fp32 side (q, then p) is split into
 //     parts of the cache's type, whose products land in rows 0-7 (part 1) and 8-15 (part 2) of the same tile:
-//       f16:  2 parts of 11 bits, q scaled by a power of two per head to use f16's range, p in [0, 2^13];
+//       f16:  2 parts of 11 bits, q scaled by a power of two per head to use f16's range, p in [0, 2^13] relative to the
+//             head's largest score in the step;
 //       bf16: 3 parts of 8 bits, the third as a second product, or in rows 4-7 where the tile has at most four heads
 //             (half the matrix instructions: 32 ragged rows 20.2 -> 18.2 us of GPU time);
 //       f32:  tf32 halves, q.k = qh.kh + ql.kh + qh.kl (and p.v likewise), 11 + 11 bits.
@@ -431,12 +432,18 @@ struct Tile {
             for (int e = 0; e < S::NO / 2; e++) o[e].x *= alpha, o[e].y *= alpha;
         }
         m = mn;
-        float p[2 * S::KT];
+        // Weights as f16 parts keep 2^-38 of what they are relative to: that is the head's largest score in the step, not
+        // its running maximum, so that a step of small weights and large values keeps its bits; its products join the
+        // output by the step's share.
+        constexpr bool LOCAL = TYPE == KX_KV_F16;
+        const float peak = LOCAL ? (mx == -INFINITY ? 0.0f : mx) : safe, share = LOCAL ? kx::ex2_approx(mx - safe) : 1.0f;
+        float p[2 * S::KT], sum = LOCAL ? 0.0f : l;
 #pragma unroll
         for (int e = 0; e < 2 * S::KT; e++) {
-            p[e] = kx::ex2_approx((s[e] - safe) + off);  // the maximum's is 2^off, however large the scores are
-            l += p[e];
+            p[e] = kx::ex2_approx((s[e] - peak) + off);  // the largest is 2^off, however large the scores are
+            sum += p[e];
         }
+        l = LOCAL ? fmaf(sum, share, l) : sum;
         // p.v: column 2 t (2 t + 1) of n-tile (k, e) is element e of chunk 8 k + t (+ 4); row t + 4 x of the step is x-th
         const uint8_t* vrow = src + S::TILE + t * S::PITCH;
         const int vch[2] = {(perm ^ t) << 4, (perm ^ t ^ 4) << 4};
@@ -487,7 +494,8 @@ struct Tile {
                         if constexpr (!FEW) mma_bf16(d, pa[2], 0, pb[2], 0, b0, b1);
                         mma_bf16(d, pa[0], pa[1], pb[0], pb[1], b0, b1);
                     }
-                    o[k * 8 + e] = add2(o[k * 8 + e], add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])));
+                    const float2 pv = add2(make_float2(d[0], d[1]), make_float2(d[2], d[3]));
+                    o[k * 8 + e] = LOCAL ? kx::fma2(pv, make_float2(share, share), o[k * 8 + e]) : add2(o[k * 8 + e], pv);
                 }
             }
         }

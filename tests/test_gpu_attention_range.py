@@ -165,3 +165,26 @@ def test_tiles_of_far_values_under_small_weights(kx, Rq, S, dk, dv, far, drop): 
         tol = math.expm1(2 * 3 * 40 * 2.0**-24) + 2.0**-18
         assert float(((got - (p @ v)[:, None]).abs() / size[:, None, None]).max()) <= tol
         assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("keys", [90, 6001])
+@pytest.mark.parametrize("small,drop", [(2.0**-14, -20.75), (2.0**-20, -24.25), (2.0**-2, -17.375), (2.0**-10, -24.25), (2.0**-14, -27.75)])
+def test_steps_of_far_values_under_small_weights_over_the_cache(kx, dtype, keys, small, drop):  # noqa: F811
+    """Pairs of 16-key steps with values of 2^15 under weights of about e^drop, in turn with pairs of small values under
+    large weights: the output keeps its bits relative to sum p|v|. Tolerance as for the prompt's tiles."""
+    for first in (0, 1):
+        g = torch.Generator().manual_seed(keys)
+        high = (torch.arange(keys) // 32) % 2 == first
+        scores = torch.randint(-16, 1, (2, keys), generator=g) / 8 + torch.where(high, drop, 0.0)
+        v = (1 + torch.rand(2, keys, 72, generator=g)) * torch.randn(2, keys, 72, generator=g).sign()
+        v = (v * torch.where(high, 2.0**15, small)[:, None]).half().float().clamp(-65504, 65504)  # 65536 is not an f16 number
+        c = scored(dtype, scores, v, group=3)
+        got = c.run(kx, scale=1.0).view(2, 3, 72).cpu().double()
+        p = torch.softmax(scores.double(), 1)
+        tol = math.expm1(2 * 3 * 40 * 2.0**-24) + 2.0**-18
+        for r in range(2):
+            stored = torch.from_numpy(c.host[r][1][:, 0])
+            size = p[r] @ stored.abs().amax(1)
+            assert float((got[r] - p[r] @ stored).abs().max() / size) <= tol
+        assert int(c.status) == 0
