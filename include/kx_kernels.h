@@ -2,8 +2,8 @@
  *
  * Plain device pointers, sizes and a cudaStream_t passed as void*; no CUDA or torch types. All matrices
  * are row-major with an explicit leading dimension (elements). Every function returns 0 when the launch
- * was accepted and -1 on bad arguments or a launch error. Kernels whose waits are bounded write
- * KX_STATUS_TIMEOUT into *status (device memory, may be NULL) instead of hanging.
+ * was accepted and -1 on bad arguments or a launch error. Kernels whose waits are bounded OR
+ * KX_STATUS_TIMEOUT into *status (device memory, may be NULL) instead of hanging; bits that are there stay.
  * Each entry names the reference computation it replaces (KERNIX reference file:line).
  */
 #ifndef KX_KERNELS_H
@@ -89,7 +89,7 @@ KERNIX_API int kx_linear_i8_noalloc(const float* x, int ldx, int rows, int k, co
  * command-buffer error handling, src/kernix_metal.m:259-263, which turns a failed GPU command into -1): one warp
  * waits on an mbarrier with the library's wait helper and a limit of limit_ns (at most 2 s). arrive = 1: the
  * barrier completes and *status is left as it was; arrive = 0: nothing arrives, the wait gives up after limit_ns
- * and writes KX_STATUS_TIMEOUT (1) to *status, and the launch ends normally. *waited_ns: time spent waiting.
+ * and ORs KX_STATUS_TIMEOUT (1) into *status, and the launch ends normally. *waited_ns: time spent waiting.
  * Device pointers; returns -1 on bad arguments or a launch error. */
 KERNIX_API int kx_probe_bounded_wait(int arrive, unsigned long long limit_ns, int* status, unsigned long long* waited_ns,
                                      void* stream);

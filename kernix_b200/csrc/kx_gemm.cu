@@ -377,7 +377,7 @@ __device__ __forceinline__ bool q_wait_count(const uint32_t* cnt, uint32_t targe
         if (*abort) return false;
         if ((spin & 63) == 63 && kx::globaltimer() - t0 > KX_WAIT_NS) {
             *abort = 1;
-            if (status) atomicExch(status, KX_STATUS_TIMEOUT);
+            if (status) atomicOr(status, KX_STATUS_TIMEOUT);
             return false;
         }
     }

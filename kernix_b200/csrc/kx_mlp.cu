@@ -104,7 +104,7 @@ __device__ bool grid_barrier(uint32_t* bar, uint32_t target, int* status, int* s
             for (uint32_t spin = 0; static_cast<int>(kx::ld_acquire_gpu(bar + 1) - target) < 0; spin++) {
                 if ((spin & 15) == 15) {
                     if (kx::globaltimer() - t0 > KX_WAIT_NS) {
-                        if (status) atomicExch(status, KX_STATUS_TIMEOUT);
+                        if (status) atomicOr(status, KX_STATUS_TIMEOUT);
                         ok = false;
                         break;
                     }

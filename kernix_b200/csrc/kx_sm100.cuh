@@ -69,7 +69,7 @@ __device__ __forceinline__ bool mbar_wait_for(uint64_t* bar, uint32_t parity, vo
         if ((spin & 63) == 63) {
             if (globaltimer() - t0 > limit_ns) {
                 *abort = 1;
-                if (status) atomicExch(status, KX_STATUS_TIMEOUT);
+                if (status) atomicOr(status, KX_STATUS_TIMEOUT);
                 return false;
             }
             __nanosleep(64);

@@ -188,3 +188,12 @@ def test_steps_of_far_values_under_small_weights_over_the_cache(kx, dtype, keys,
             size = p[r] @ stored.abs().amax(1)
             assert float((got[r] - p[r] @ stored).abs().max() / size) <= tol
         assert int(c.status) == 0
+
+
+def test_a_timeout_keeps_the_status_bits(kx):  # noqa: F811
+    """one status word for a step's calls: a wait that gives up adds its bit to those that are there"""
+    status = torch.full((1,), 2 | 4, dtype=torch.int32, device="cuda")
+    waited = torch.zeros(1, dtype=torch.int64, device="cuda")
+    kx.call("kx_probe_bounded_wait", 0, 5_000_000, status.data_ptr(), waited.data_ptr(), None)
+    torch.cuda.synchronize()
+    assert int(status) == 1 | 2 | 4
