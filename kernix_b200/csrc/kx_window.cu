@@ -32,7 +32,8 @@
 //  Tiles that the parts cannot hold (NaN, infinities, magnitudes from 2^40 on; a key or value row whose largest element is
 //  below 2^-14 of the tile's; nothing but values below 2^-40) are flagged by k_win_prep; a CTA that would read a flagged tile, or has such a q, computes
 //  its rows with plain fp32 code that reads only what each row sees.
-// Every wait is bounded; a timeout records KX_STATUS_TIMEOUT in the status word and the CTA stops.
+// Every wait is bounded; a timeout records KX_STATUS_TIMEOUT in the status word and the CTA stops: its rows are left as they
+// were, or, where a block is split, become NaN.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -704,7 +705,8 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                 const float mm = fmaxf(m, his[0]), safe = mm == -INFINITY ? 0.0f : mm;
                 float f0 = kx::ex2_approx(m - safe), f1 = kx::ex2_approx(his[0] - safe);
                 const float den = f0 * l + f1 * his[1];
-                if (SPLIT && grp == 0) part()->ml[r] = make_float2(mm, den);
+                // after a timeout the part's rows are not written: a sum of NaN makes the joined rows NaN
+                if (SPLIT && grp == 0) part()->ml[r] = ctl.abort ? make_float2(0.0f, NAN) : make_float2(mm, den);
                 const float inv = SPLIT ? 1.0f : den == 0.0f ? 0.0f : 1.0f / den;
                 f0 *= inv, f1 *= inv;
                 float* z = half + (grp * WN_ROWS + r) * P;
