@@ -137,7 +137,8 @@ __host__ __device__ inline size_t part_bytes(int dv) { return sizeof(PartHead) +
 __device__ __forceinline__ Tiles tiles_of(const WinArgs& A, int p0, int p1) {
     Tiles t{0, 0, 0};
     if (p1 < 0) return t;
-    const int w0 = A.window > 0 ? max(0, p0 - A.window + 1) : 0, s0 = min(A.sinks, w0);
+    // max: the first of very many queries may lie 2^31 before the first key
+    const int w0 = A.window > 0 ? max(0, max(p0, 0) - A.window + 1) : 0, s0 = min(A.sinks, w0);
     t.na = (s0 + WN_KEYS - 1) / WN_KEYS;
     t.b0 = max(t.na, w0 / WN_KEYS);
     t.end = p1 / WN_KEYS + 1;
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(256) k_win_prep(const __grid_constant__ WinArg
     const float* vr = A.v + (static_cast<long>(b) * A.S + j0) * A.ldv + h * A.dv;
     // a warp per row, all of its rows asked for at once; rows behind the last key and rows that no query sees (behind the
     // first tokens, before the first query's window) are zero, so that they touch neither the scales nor the flag
-    const int back = kl - ql - A.window;  // the last position before every window
+    const int back = max(kl - ql, 0) - A.window;  // the last position before every window
     float4 kx4[WN_KEYS / 8], vx4[WN_KEYS / 8];
 #pragma unroll
     for (int u = 0; u < WN_KEYS / 8; u++) {
@@ -870,7 +871,7 @@ int kx_attention_window(const float* q, int ldq, const float* k, int ldk, const 
     A.chunks = (A.G + A.per_chunk - 1) / A.per_chunk;
     A.tiles = L.tiles, A.ka = L.ka, A.vp = L.vp, A.block = L.block;
     A.qt = WN_ROWS / A.per_chunk;
-    A.qtiles = (Rq + A.qt - 1) / A.qt;
+    A.qtiles = (Rq - 1) / A.qt + 1;
     A.scale2 = (scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(dk)) : scale) * 1.4426950408889634f;
     const auto vec = [](const float* p, int ld, int d) { return ((ld | d) & 3) == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
     A.vecq = vec(q, ldq, dk), A.veck = vec(k, ldk, dk), A.vecv = vec(v, ldv, dv);

@@ -197,3 +197,17 @@ def test_a_timeout_keeps_the_status_bits(kx):  # noqa: F811
     kx.call("kx_probe_bounded_wait", 0, 5_000_000, status.data_ptr(), waited.data_ptr(), None)
     torch.cuda.synchronize()
     assert int(status) == 1 | 2 | 4
+
+
+@pytest.mark.parametrize("window", [0, 40])
+def test_the_most_query_rows(kx, window):  # noqa: F811
+    """Rq of 2^31 - 1, of which the sample has a few: the rows behind them are not there"""
+    c = Case(1, 150, 200, 2, 1, 32, 32, window=window, sinks=1, q_len=[150], k_len=[200])
+    want = c.run(kx).clone()
+    c.args(kx)
+    dims, c.dims = c.dims, (1, 2**31 - 1) + c.dims[2:]
+    c.launch(kx, sp())
+    torch.cuda.synchronize()
+    c.dims = dims
+    c.check(c.ctx)
+    assert torch.equal(c.ctx, want) and int(c.status) == 0
