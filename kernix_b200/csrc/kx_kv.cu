@@ -568,8 +568,8 @@ int kx_kv_append(const kx_kv* c, int layer, const float* k, int ldk, const float
     int lanes = 0;
     while (lanes < 8 && 1 << lanes < chunks) lanes++;
     // 16 rows per thread, 65535 CTAs per slot at most
-    const int rb = std::max(16 << (8 - lanes), (rows + 65534) / 65535);
-    const dim3 grid(c->n_seqs, (rows + rb - 1) / rb);
+    const int rb = std::max(16 << (8 - lanes), (rows - 1) / 65535 + 1);
+    const dim3 grid(c->n_seqs, (rows - 1) / rb + 1);
     const bool vec = ((ldk | ldv) & 3) == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
     const long sz = kx::kv_elem_bytes(c->type);
     const long k_off = layer ? layer * c->k_layer * sz : 0, v_off = layer ? layer * c->v_layer * sz : 0;

@@ -5,6 +5,7 @@ import math
 import numpy as np
 import pytest
 
+from kv_model import ref
 from test_gpu_window import Case, kx, sp  # noqa: F401 (kx: fixture)
 
 torch = pytest.importorskip("torch")
@@ -211,3 +212,19 @@ def test_the_most_query_rows(kx, window):  # noqa: F811
     c.dims = dims
     c.check(c.ctx)
     assert torch.equal(c.ctx, want) and int(c.status) == 0
+
+
+@pytest.mark.parametrize("rows", [2**31 - 1, 2**31 - 65535, 65535 * 16 + 1])
+def test_append_with_the_most_rows(kx, rows):  # noqa: F811
+    """room for up to 2^31 - 1 rows per slot, of which the first slot has 13: the others are not there"""
+    from test_gpu_kv import Pair
+    out = []
+    for r in (13, rows):
+        p = Pair(kx, 2, 4, 12, 8, heads=2, dk=16, dv=24, dtype="f32")
+        p.extend([13, 0])
+        x, count = torch.randn(13, 48, generator=torch.Generator().manual_seed(2)).cuda(), p.ints([13, 0])
+        kx.call("kx_kv_append", ref(p.c), 0, x.data_ptr(), 48, x.data_ptr(), 48, count.data_ptr(), r, p.status.data_ptr(), sp())
+        torch.cuda.synchronize()
+        assert int(p.status) == 0
+        out.append((p.bits(p.k), p.bits(p.v)))
+    assert np.array_equal(out[0][0], out[1][0]) and np.array_equal(out[0][1], out[1][1])
