@@ -88,6 +88,8 @@ struct Span {
     bool bad;           // the row's slot or length is out of range
 };
 template <int KS>
+__device__ __forceinline__ int steps_of(int keys) { return static_cast<int>((static_cast<unsigned>(keys) + KS - 1) / KS); }
+template <int KS>
 __device__ __forceinline__ Span span_of(const PagedArgs& A, int row, int* slot) {
     Span sp;
     const int s = A.seqs ? A.seqs[row] : row;
@@ -102,9 +104,9 @@ __device__ __forceinline__ Span span_of(const PagedArgs& A, int row, int* slot) 
     sp.len = len;
     sp.w0 = A.window > 0 && len > A.window ? len - A.window : 0;
     sp.s0 = min(A.sinks, sp.w0);
-    sp.na = (sp.s0 + KS - 1) / KS;
+    sp.na = steps_of<KS>(sp.s0);
     sp.b0 = max(sp.na, sp.w0 / KS);
-    sp.steps = max(1, sp.na + (len + KS - 1) / KS - sp.b0);  // a row that sees nothing still has its zeros to write
+    sp.steps = max(1, sp.na + steps_of<KS>(len) - sp.b0);  // a row that sees nothing still has its zeros to write
     return sp;
 }
 
@@ -219,7 +221,7 @@ struct Cursor {
     // every key of the step is seen
     __device__ __forceinline__ bool whole() const {
         const int j = first_key();
-        return j + S::KS <= sp.len && (j >= sp.w0 || j + S::KS <= sp.s0);
+        return sp.len - j >= S::KS && (j >= sp.w0 || sp.s0 - j >= S::KS);
     }
     __device__ __forceinline__ bool visible(int j) const { return j < sp.len && (j < sp.s0 || j >= sp.w0); }
 };
@@ -232,6 +234,8 @@ struct Feed {
     const int32_t* table;
     const char *kb, *vb;
     int ids, base;  // ids: table[base + lane]
+
+    __device__ __forceinline__ bool held(int entry) const { return static_cast<unsigned>(entry) - static_cast<unsigned>(base) < 32u; }
 
     __device__ __forceinline__ void unit(const PagedArgs& A, const Cursor<TYPE, D>& c) {
         const int kvh = c.unit / A.chunks;
@@ -247,9 +251,9 @@ struct Feed {
     // that are not seen become zero. false: a page that a visible key lies on is not there; its row is zero, too.
     __device__ __forceinline__ bool issue(const PagedArgs& A, const Cursor<TYPE, D>& c, uint32_t dst, int nck, int ncv, int shift) {
         const int lane = threadIdx.x & 31, first = c.first_key(), lr = lane >> 3, lc = lane & 7;
-        if ((first >> shift) < base || ((first + S::KS - 1) >> shift) >= base + 32) {
+        if (!held(first >> shift) || !held((first + S::KS - 1) >> shift)) {
             base = first >> shift;
-            ids = base + lane <= (c.sp.len - 1) >> shift ? __ldcg(table + base + lane) : 0;
+            ids = lane <= ((c.sp.len - 1) >> shift) - base ? __ldcg(table + base + lane) : 0;
         }
         // rows lr + 4 y, chunks lc + 8 x
         const uint32_t to[2] = {dst + lr * S::PITCH + ((lc ^ lr) << 4), dst + lr * S::PITCH + ((lc ^ lr ^ 4) << 4)};
@@ -955,7 +959,7 @@ int kx_attention_paged(const kx_kv* c, int layer, const float* q, int ldq, int H
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0)
         return -1;
     const long units = static_cast<long>(n) * c->heads * A.chunks;
-    if (units > INT32_MAX) return -1;
+    if (units > INT32_MAX - PG_THREADS) return -1;  // rows are counted in steps of a CTA
     // the most steps a unit can have
     const int ks = c->type == KX_KV_F32 ? 8 : 16;
     long keys = static_cast<long>(c->max_pages) * c->page;

@@ -228,3 +228,41 @@ def test_append_with_the_most_rows(kx, rows):  # noqa: F811
         assert int(p.status) == 0
         out.append((p.bits(p.k), p.bits(p.v)))
     assert np.array_equal(out[0][0], out[1][0]) and np.array_equal(out[0][1], out[1][1])
+
+
+@pytest.mark.parametrize("dtype,page,max_pages", [("f16", 8, 2**28 - 1), ("f16", 16, 2**27 - 1), ("f32", 1, 2**31 - 1025), ("bf16", 1, 2**31 - 1025)])
+def test_sequences_of_almost_2_to_31_tokens(kx, dtype, page, max_pages):  # noqa: F811
+    """A table that names few pages again and again: 0 for the first half, 1 for the second, 2 for the last 16 tokens, 3 for
+    the first 16. A lane adds up to 2^19 terms (2^31 over 1184 warps of four lanes): an fp32 sum is off by 2^19 2^-24 of itself at most,
+    the output by twice that."""
+    import test_gpu_paged as tp
+    length, d, n = max_pages * page, 8, 16 // page if page < 16 else 1
+    g = torch.Generator().manual_seed(1)
+    k = torch.randn(4 * n, page, d, generator=g).to(tp.DTYPES[dtype])
+    v = (torch.randn(4 * n, page, d, generator=g) / 8 + torch.tensor([1.0, 3.0, 7.0, -5.0]).repeat_interleave(n)[:, None, None]).to(tp.DTYPES[dtype])
+    table = torch.empty(1, max_pages, dtype=torch.int32, device="cuda")
+    for at, which in ((0, 0), (max_pages // 2, 1)):
+        table[0, at:] = which * n
+    table[0, -n:] = torch.arange(2 * n, 3 * n, dtype=torch.int32, device="cuda")
+    table[0, :n] = torch.arange(3 * n, 4 * n, dtype=torch.int32, device="cuda")
+    lens = torch.tensor([length], dtype=torch.int32, device="cuda")
+    c = tp.Case.__new__(tp.Case)
+    c.lens, c.heads, c.G, c.dk, c.dv, c.page, c.layer, c.dtype = [length], 1, 2, d, d, page, 0, dtype
+    c.k, c.v = k.cuda()[None, :, None].contiguous(), v.cuda()[None, :, None].contiguous()
+    c.q, c.table, c.d_lens = torch.randn(1, 2 * d, generator=g) / 4, table, lens
+    c.refs, c.status = torch.ones(4 * n, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    q = c.q.double().view(2, d)
+    rows = lambda ids: [x.double()[ids].reshape(-1, d) for x in (k, v)]  # noqa: E731
+    (k0, v0), (k2, v2), (k3, v3) = (rows(list(range(i * n, i * n + n))) for i in (0, 2, 3))
+    # the first tokens and the window's
+    c.window, c.sinks = 5, 3
+    got = c.run(kx).view(2, d).double().cpu()
+    want, tol = tp.exact(q.numpy(), torch.cat([k3[:3], k2[-5:]]).numpy(), torch.cat([v3[:3], v2[-5:]]).numpy(), 1 / math.sqrt(d))
+    assert np.all(np.abs(got.numpy() - want) <= tol)
+    # all of them: page 0 and page n half each, the 32 others do not show
+    c.window, c.sinks = 0, 0
+    got = c.run(kx).view(2, d).double().cpu()
+    kk, vv = (torch.cat([x.double()[0], x.double()[n]]) for x in (k, v))
+    want = torch.softmax(q @ kk.T / math.sqrt(d), 1) @ vv
+    assert float((got - want).abs().max()) <= 2 * (2.0**19 * 2.0**-24) * 3.5, (got, want)
+    assert int(c.status) == 0
