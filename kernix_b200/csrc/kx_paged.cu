@@ -927,7 +927,7 @@ size_t kx_attention_paged_ws(const kx_kv* c, int H, int n) {
 int kx_attention_paged(const kx_kv* c, int layer, const float* q, int ldq, int H, const int32_t* seqs, int n, int window, int sinks,
                        float scale, float* ctx, int ldc, void* ws, size_t ws_bytes, int* status, void* stream) {
     const size_t need = kx_attention_paged_ws(c, H, n);
-    if (need == 0 || layer < 0 || layer >= c->layers || sinks < 0 || !std::isfinite(scale)) return -1;
+    if (need == 0 || layer < 0 || layer >= c->layers || sinks < 0 || !std::isfinite(scale * 1.4426950408889634f)) return -1;
     if (!seqs && n > c->n_seqs) return -1;
     if (n == 0) return 0;
     if (!q || !ctx || ldq < static_cast<long>(H) * c->dk || ldc < static_cast<long>(H) * c->dv) return -1;

@@ -852,7 +852,7 @@ int kx_attention_window(const float* q, int ldq, const float* k, int ldk, const 
                         int S, int H, int Hkv, int dk, int dv, const int32_t* q_len, const int32_t* k_len, int window, int sinks,
                         float scale, void* ws, size_t ws_bytes, int* status, void* stream) {
     WinLayout L;
-    if (!layout_of(B, S, Hkv, dk, dv, &L) || Rq < 0 || H < 1 || H % Hkv || sinks < 0 || !std::isfinite(scale)) return -1;
+    if (!layout_of(B, S, Hkv, dk, dv, &L) || Rq < 0 || H < 1 || H % Hkv || sinks < 0 || !std::isfinite(scale * 1.4426950408889634f)) return -1;
     if (B == 0 || Rq == 0) return 0;
     if (!q || !k || !v || !ctx || ldq < static_cast<long>(H) * dk || ldk < static_cast<long>(Hkv) * dk ||
         ldv < static_cast<long>(Hkv) * dv || ldc < static_cast<long>(H) * dv)
