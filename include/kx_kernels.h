@@ -257,7 +257,7 @@ KERNIX_API int kx_attention(const float* q, int ldq, const float* k, int ldk, co
  * An empty cache has lens = 0, refs = 0, table = -1; the entry points below keep these consistent.
  * Requirements, else -1: page a power of two up to 1024; dk * size and dv * size multiples of 16 bytes, dk, dv <= 1024;
  * k, v and all strides * size multiples of 16 bytes; pages (and layers) that do not overlap;
- * max_pages * page < 2^31; heads * page * dk and heads * page * dv <= 2^28. Calls that change a cache are ordered on one
+ * max_pages * page < 2^31, max_pages < 2^31 - 1024; n_pages, n_seqs <= 2^30; heads * page * dk and heads * page * dv <= 2^28. Calls that change a cache are ordered on one
  * stream (or by events) with those that use it.
  *
  * Requests live in device memory, so a kernel checks them: what it refuses it leaves out, memory-safely, and ORs a bit
