@@ -319,9 +319,9 @@ KERNIX_API int kx_kv_compact(const kx_kv* c, int32_t* n_live, void* ws, size_t w
  * their pages): row i, i < n, is the last token (position lens - 1, appended before) of slot seqs[i] (seqs NULL: slot i),
  * its H query heads in q + i * ldq (H * dk floats); query head h reads key-value head h / (H / heads). It sees key j
  * when window <= 0, or j > lens - 1 - window, or j < sinks. ctx + i * ldc receives H * dv floats. scale 0 means
- * 1/sqrt(dk). A row with seqs[i] < 0 is left as it was, one whose slot holds no tokens becomes 0, and one whose slot,
+ * 1/sqrt(dk); |scale| < 2.3e38. A row with seqs[i] < 0 is left as it was, one whose slot holds no tokens becomes 0, and one whose slot,
  * length or (visible) pages are out of range becomes NaN and is reported. Keys and values that are not seen do not affect
- * results, whatever they hold; those that are have to be finite and, in an fp32 cache, below 2^127 (a head that sees an
+ * results, whatever they hold; q and those that are have to be finite and, q and an fp32 cache, below 2^127 (a head that sees an
  * infinite key becomes NaN, a column with an infinite value NaN). H a multiple of heads, dk, dv <= 128. q and ctx must not
  * overlap each other or the cache. Accuracy is fp32's; against an f16 cache q keeps 2^-22 of itself, or 2^-38 of its head's
  * largest element where that is more, and a weight 2^-22 of itself or 2^-38 of the largest among its 16 keys (positions 16 i to

@@ -330,7 +330,8 @@ struct Tile {
                 x[k * S::EPC + e + 3] = f.w;
             }
         qscale = A.scale2;
-        off = 0.0f;
+        // weights up to 2^off: below 1 / len, so that no sum of weighted values passes the largest value
+        off = static_cast<float>(__clz(c.sp.len) - 32);
         if constexpr (TYPE == KX_KV_F16) {
             // |q| < 2^14 after the scaling; parts keep 22 bits of what is above 2^-17 of the head's largest element
             float top = 0.0f;

@@ -319,6 +319,8 @@ __device__ __noinline__ void plain_rows(const WinArgs& A, int b, int kvh, int he
 #pragma unroll
         for (int x = 0; x < 4; x++) q[x] = lane + 32 * x < A.dk ? qr[lane + 32 * x] * A.scale2 : 0.0f;
         const int w0 = A.window > 0 ? max(0, p - A.window + 1) : 0, s0 = min(A.sinks, w0);
+        // weights up to 2^off: below 1 / (p + 1), so that no sum of weighted values passes the largest value
+        const float off = static_cast<float>(__clz(p + 1) - 32);
         for (int j = s0 > 0 ? 0 : w0; j <= p; j = j + 1 == s0 ? w0 : j + 1) {
             const float* kr = A.k + (static_cast<long>(b) * A.S + j) * A.ldk + kvh * A.dk;
             const float* vr = A.v + (static_cast<long>(b) * A.S + j) * A.ldv + kvh * A.dv;
@@ -330,7 +332,7 @@ __device__ __noinline__ void plain_rows(const WinArgs& A, int b, int kvh, int he
             for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(FULL, s, d);
             // a NaN score stays: it makes the sum NaN
             const float mn = fmaxf(m, s), safe = mn == -INFINITY ? 0.0f : mn;
-            const float back = m == mn ? 1.0f : kx::ex2_approx(m - safe), e = kx::ex2_approx(s - safe);
+            const float back = m == mn ? 1.0f : kx::ex2_approx(m - safe), e = kx::ex2_approx((s - safe) + off);
             m = mn;
             l = l * back + e;
 #pragma unroll

@@ -266,3 +266,34 @@ def test_sequences_of_almost_2_to_31_tokens(kx, dtype, page, max_pages):  # noqa
     want = torch.softmax(q @ kk.T / math.sqrt(d), 1) @ vv
     assert float((got - want).abs().max()) <= 2 * (2.0**19 * 2.0**-24) * 3.5, (got, want)
     assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("keys", [1, 2, 15, 90, 4000])
+def test_the_largest_values_over_the_cache(kx, dtype, keys):  # noqa: F811
+    """nearly equal weights over values just below 2^127: the output is one of them, not the overflow of their sum"""
+    g = torch.Generator().manual_seed(keys)
+    scores = torch.randint(-4, 1, (2, keys), generator=g) / 8
+    v = 2.0**126 * (1.5 + torch.rand(2, keys, 40, generator=g, dtype=torch.float64) / 4)
+    v[1] *= torch.randn(keys, 40, generator=g).sign()
+    c = scored(dtype, scores, v)
+    got = c.run(kx, scale=1.0).view(2, 2, 40).cpu().double()
+    for r in range(2):
+        want = torch.softmax(scores[r].double(), 0) @ torch.from_numpy(c.host[r][1][:, 0])
+        assert float((got[r] - want).abs().max()) <= 2.0**-17 * 2.0**127
+    assert int(c.status) == 0
+
+
+@pytest.mark.parametrize("S", [2, 130, 1000])
+def test_the_largest_values_of_a_prompt(kx, S):  # noqa: F811
+    """the plain way"""
+    c = Case(1, S, S, 2, 1, 32, 32, window=700, sinks=2, seed=8)
+    g = torch.Generator().manual_seed(S)
+    c.v = 2.0**127 * (1.5 + torch.rand(c.v.shape, generator=g, dtype=torch.float64) / 4).float()
+    c.v[0, ::3] *= -1
+    got = c.run(kx).double().view(S, 2, 32)
+    seen = c.seen(0).cuda()
+    for h in range(2):
+        s = (c.q[0, :, h].double().cuda() @ c.k[0, :, 0].double().cuda().T / math.sqrt(32)).masked_fill(~seen, -math.inf)
+        want = torch.softmax(s, 1) @ c.v[0, :, 0].double().cuda()
+        assert float((got[:, h] - want).abs().max()) <= 2.0**-17 * 2.0**128
