@@ -134,14 +134,6 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], uint32_t a0, uint32_t a1
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(d[0]), "f"(d[1]), "f"(d[2]), "f"(d[3]));
 }
 
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("add.rn.f32x2 %0, %1, %2;"
-        : "=l"(reinterpret_cast<uint64_t&>(r))
-        : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
-    return r;
-}
-
 // two fp32 values as PARTS pairs of the 16-bit type, the value = the sum of its parts up to the last one's rounding
 template <int TYPE>
 __device__ __forceinline__ uint32_t pack2(float a, float b, float* ra, float* rb) {
@@ -466,7 +458,7 @@ struct Tile {
                     const uint32_t v0 = tf32_of(__uint_as_float(wa[e]), &l0), v1 = tf32_of(__uint_as_float(wb[e]), &l1);
                     mma_tf32(d, h0, 0, h1, 0, __float_as_uint(l0), __float_as_uint(l1));
                     mma_tf32(d, h0, __float_as_uint(q0), h1, __float_as_uint(q1), v0, v1);
-                    o[k * 4 + e] = add2(o[k * 4 + e], add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])));
+                    o[k * 4 + e] = kx::add2(o[k * 4 + e], kx::add2(make_float2(d[0], d[1]), make_float2(d[2], d[3])));
                 }
             }
         } else {
@@ -499,8 +491,8 @@ struct Tile {
                         if constexpr (!FEW) mma_bf16(d, pa[2], 0, pb[2], 0, b0, b1);
                         mma_bf16(d, pa[0], pa[1], pb[0], pb[1], b0, b1);
                     }
-                    const float2 pv = add2(make_float2(d[0], d[1]), make_float2(d[2], d[3]));
-                    o[k * 8 + e] = LOCAL ? kx::fma2(pv, make_float2(share, share), o[k * 8 + e]) : add2(o[k * 8 + e], pv);
+                    const float2 pv = kx::add2(make_float2(d[0], d[1]), make_float2(d[2], d[3]));
+                    o[k * 8 + e] = LOCAL ? kx::fma2(pv, make_float2(share, share), o[k * 8 + e]) : kx::add2(o[k * 8 + e], pv);
                 }
             }
         }
