@@ -650,15 +650,22 @@ __global__ void __launch_bounds__(WN_THREADS, 1) k_win_main(const __grid_constan
                 const float share = kx::ex2_approx(peak - (m == -INFINITY ? 0.0f : m));
                 const bool far = __any_sync(FULL, fabsf(safe) >= WN_FAR);
                 const float mul = far ? 1.0f : f, shift = far ? 13.0f : 13.0f - safe;
+                if (far) {
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        uint32_t(&x)[32] = s[D > 64 ? 0 : c];
+                        if (D > 64) load(c, x);
+#pragma unroll
+                        for (int y = 0; y < 32; y++) x[y] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(x[y]), f), -safe));
+                        if (D > 64) kx::tmem_st32(sm + c * 32, x);
+                    }
+                    if (D > 64) kx::tmem_st_wait();
+                }
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
                     uint32_t(&x)[32] = s[D > 64 ? 0 : c];
                     if (D > 64) load(c, x);
-                    if (far) {
-#pragma unroll
-                        for (int y = 0; y < 32; y++) x[y] = __float_as_uint(__fadd_rn(__fmul_rn(__uint_as_float(x[y]), f), -safe));
-                    }
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int y = 0; y < 32; y += 2) {
