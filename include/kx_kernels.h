@@ -295,7 +295,9 @@ KERNIX_API int kx_kv_extend(const kx_kv* c, const int32_t* want, int32_t* grante
 
 /* The last count[s] tokens of every slot s (positions lens[s] - count[s] .. lens[s] - 1) of one layer from fp32 rows
  * s * rows + i, i < count[s] (<= rows; <= 0: none): heads * dk floats of k at leading dimension ldk, heads * dv of v at
- * ldv, rounded to the cache's type (to nearest even). Rows i >= count[s] are not read. k and v must not overlap the pools. */
+ * ldv, rounded to the cache's type (to nearest even). Rows i >= count[s] are not read. k and v must not overlap the pools. The
+ * tokens' pages are the slot's alone (append before a fork shares them): what lands in a shared page is there for all of its
+ * sequences, and of two slots that write the same token of it in one call either's row stays. */
 KERNIX_API int kx_kv_append(const kx_kv* c, int layer, const float* k, int ldk, const float* v, int ldv, const int32_t* count,
                             int rows, int* status, void* stream);
 
@@ -325,8 +327,7 @@ KERNIX_API int kx_kv_compact(const kx_kv* c, int32_t* n_live, void* ws, size_t w
  * infinite key becomes NaN, a column with an infinite value NaN). H a multiple of heads, dk, dv <= 128. q and ctx must not
  * overlap each other or the cache. Accuracy is fp32's; against an f16 cache q keeps 2^-22 of itself, or 2^-38 of its head's
  * largest element where that is more, and a weight 2^-22 of itself or 2^-38 of the largest among its 16 keys (positions 16 i to
- * 16 i + 15). ws: kx_attention_paged_ws bytes of device workspace (0: the arguments are
- * invalid), to be shared under kx_kv_ws's rules. Results do not depend on timing: the same call on the same contents
+ * 16 i + 15). ws: kx_attention_paged_ws bytes of device workspace (0: the arguments are invalid), to be shared under kx_kv_ws's rules. Results do not depend on timing: the same call on the same contents
  * gives the same bits. */
 KERNIX_API size_t kx_attention_paged_ws(const kx_kv* c, int H, int n);
 KERNIX_API int kx_attention_paged(const kx_kv* c, int layer, const float* q, int ldq, int H, const int32_t* seqs, int n, int window,
@@ -340,13 +341,14 @@ KERNIX_API int kx_attention_paged(const kx_kv* c, int layer, const float* q, int
  * (window <= 0 or j > t - window or j < sinks). ctx rows b * Rq + i (ldc, H * dv floats); a row that sees nothing (t < 0)
  * becomes 0, rows i >= q_len are left as they were; a sample whose lengths are out of range is reported
  * (KX_STATUS_BAD_REQUEST) and its Rq rows become NaN. Query head h reads key-value head h / (H / Hkv). scale 0 means
- * 1/sqrt(dk). dk, dv <= 128, H a multiple of Hkv. q, k, v must not overlap ctx or ws. ws: kx_attention_window_ws bytes
+ * 1/sqrt(dk); |scale| < 2.3e38. dk, dv <= 128, H a multiple of Hkv. q, k, v must not overlap ctx or ws. ws: kx_attention_window_ws bytes
  * of device workspace (0: the arguments are invalid), 128-byte aligned, shared under kx_kv_ws's rules. Key and value
- * rows that no query of the sample sees do not affect results, whatever they hold. Accuracy is fp32's: products keep 2^-22
- * of their operands, where an element of q (k or v) is not below 2^-16 of the largest in its row (in its 64 rows), or a
- * weight not below 2^-16 of the largest that its row has among those 64 keys; below that they keep 2^-38 of that largest. Blocks of 128 rows that see NaN, infinities, magnitudes of 2^40 and more, rows of
- * k or v 2^14 times above one of their neighbours, or 64 rows of v all below 2^-40, are computed by plain fp32 code, at a
- * small fraction of the speed. */
+ * rows that no query of the sample sees do not affect results, not in their last bits either, whatever they hold; a row that
+ * some queries see takes part in the roundings of its 64 neighbours. Accuracy is fp32's: products keep 2^-22 of their operands,
+ * where an element of q (k or v) is not below 2^-16 of the largest in its row (in its 64 rows), or a weight not below 2^-16 of
+ * the largest that its row has among those 64 keys; below that they keep 2^-38 of that largest. Blocks of 128 rows that see
+ * NaN, infinities, magnitudes of 2^40 and more, rows of k or v 2^14 times above one of their neighbours, or 64 rows of v all
+ * below 2^-40, are computed by plain fp32 code, 8 (128 keys a row) to 300 times slower (2500 keys). */
 KERNIX_API size_t kx_attention_window_ws(int B, int S, int Hkv, int dk, int dv);
 KERNIX_API int kx_attention_window(const float* q, int ldq, const float* k, int ldk, const float* v, int ldv, float* ctx, int ldc,
                                    int B, int Rq, int S, int H, int Hkv, int dk, int dv, const int32_t* q_len, const int32_t* k_len,

@@ -24,14 +24,18 @@
 //    work on the other's. Each group keeps a softmax of its own (maximum, sum, output); the two are joined at the end.
 //    Sums: S and a tile's P.V are at most 24 accumulated steps in the tensor core, everything longer is fp32 adds.
 //    Bound: the chain S -> softmax -> P.V of a group and, close to it, the tensor cores (for heads of 128 a tile's
-//    products are 1536 cycles of tensor work; measured 2240 per tile, in which each group's softmax is 1500 of its 4480)
+//    products are 1536 cycles of tensor work; measured 2240 per tile, in which each group's softmax is 1500 of its 4480, before
+//    the rounding of large scores and the weights per tile, which cost 1 %)
 //    plus a CTA's beginning and end, one fifth of its time. 16384 rows of 16 heads of 128 over 4 key-value heads with a
-//    window of 2048: 749 us, 345 TFLOP/s of fp32 products; three fp16 products at the measured matrix rate are 461 us.
+//    window of 2048: 884 us a call with inputs that change from call to call, 292 TFLOP/s of fp32 products, and 767 us, 336
+//    TFLOP/s, in a replayed graph on the same inputs; three fp16 products at the measured matrix rate are 461 us.
 //    One issuing thread for both products stood in its own way with heads of 64, whose products are short (a matrix
 //    instruction takes about 45 cycles to issue): 124 us against 111.
 //  Tiles that the parts cannot hold (NaN, infinities, magnitudes from 2^40 on; a key or value row whose largest element is
-//  below 2^-14 of the tile's; nothing but values below 2^-40) are flagged by k_win_prep; a CTA that would read a flagged tile, or has such a q, computes
-//  its rows with plain fp32 code that reads only what each row sees.
+//  below 2^-14 of the tile's; nothing but values below 2^-40) are flagged by k_win_prep; a CTA that would read a flagged tile,
+//  or has such a q, computes its rows with plain fp32 code that reads only what each row sees: a warp per row, one key after
+//  another. Of the 16384 rows above, one such tile of one key-value head in the middle makes it 16 ms, the first tokens' tile of
+//  one head 59 ms, of all four 197 ms.
 // Every wait is bounded; a timeout records KX_STATUS_TIMEOUT in the status word and the CTA stops: its rows are left as they
 // were, or, where a block is split, become NaN.
 #include <cuda_fp16.h>

@@ -297,3 +297,11 @@ def test_the_largest_values_of_a_prompt(kx, S):  # noqa: F811
         s = (c.q[0, :, h].double().cuda() @ c.k[0, :, 0].double().cuda().T / math.sqrt(32)).masked_fill(~seen, -math.inf)
         want = torch.softmax(s, 1) @ c.v[0, :, 0].double().cuda()
         assert float((got[:, h] - want).abs().max()) <= 2.0**-17 * 2.0**128
+
+
+@pytest.mark.parametrize("B,S", [(1, 3000), (40, 90)])
+def test_queries_without_keys(kx, B, S):  # noqa: F811
+    """samples of no keys: rows of zeros, split launches and others; the rows behind the queries are left alone"""
+    c = Case(B, 20, S, 2, 1, 64, 40, q_len=[17] * B, k_len=[0] * B)
+    ctx = c.run(kx).view(B, 20, 80)
+    assert not ctx[:, :17].any() and bool((ctx[:, 17:] == 7).all()) and int(c.status) == 0
