@@ -317,38 +317,38 @@ KERNIX_API int kx_kv_free(const kx_kv* c, const int32_t* seqs, int n, int* statu
  * the contents (every layer), references and table entries of the r-th live page from n_live on. n_live: device word. */
 KERNIX_API int kx_kv_compact(const kx_kv* c, int32_t* n_live, void* ws, size_t ws_bytes, void* stream);
 
-/* Attention of one new token per row over the cache (scaled dot products as kx_attention, keys and values read from
- * their pages): row i, i < n, is the last token (position lens - 1, appended before) of slot seqs[i] (seqs NULL: slot i),
- * its H query heads in q + i * ldq (H * dk floats); query head h reads key-value head h / (H / heads). It sees key j
- * when window <= 0, or j > lens - 1 - window, or j < sinks. ctx + i * ldc receives H * dv floats. scale 0 means
- * 1/sqrt(dk); |scale| < 2.3e38. A row with seqs[i] < 0 is left as it was, one whose slot holds no tokens becomes 0, and one whose slot,
- * length or (visible) pages are out of range becomes NaN and is reported. Keys and values that are not seen do not affect
- * results, whatever they hold; q and those that are have to be finite and, q and an fp32 cache, below 2^127 (a head that sees an
+/* Attention of one new token per row over the cache (scaled dot products as kx_attention, keys and values read from their
+ * pages): row i, i < n, is the last token (position lens - 1, appended before) of slot seqs[i] (seqs NULL: slot i), its H
+ * query heads in q + i * ldq (H * dk floats); query head h reads key-value head h / (H / heads). It sees key j when window
+ * <= 0, or j > lens - 1 - window, or j < sinks. ctx + i * ldc receives H * dv floats. scale 0 means 1/sqrt(dk); |scale| <
+ * 2.3e38. A row with seqs[i] < 0 is left as it was, one whose slot holds no tokens becomes 0, and one whose slot, length or
+ * (visible) pages are out of range becomes NaN and is reported. Keys and values that are not seen do not affect results,
+ * whatever they hold; q and those that are have to be finite and, q and an fp32 cache, below 2^127 (a head that sees an
  * infinite key becomes NaN, a column with an infinite value NaN). H a multiple of heads, dk, dv <= 128. q and ctx must not
  * overlap each other or the cache. Accuracy is fp32's; against an f16 cache q keeps 2^-22 of itself, or 2^-38 of its head's
- * largest element where that is more, and a weight 2^-22 of itself or 2^-38 of the largest among its 16 keys (positions 16 i to
- * 16 i + 15). ws: kx_attention_paged_ws bytes of device workspace (0: the arguments are invalid), to be shared under kx_kv_ws's rules. Results do not depend on timing: the same call on the same contents
- * gives the same bits. */
+ * largest element where that is more, and a weight 2^-22 of itself or 2^-38 of the largest among its 16 keys (positions 16 i
+ * to 16 i + 15). ws: kx_attention_paged_ws bytes of device workspace (0: the arguments are invalid), to be shared under
+ * kx_kv_ws's rules. Results do not depend on timing: the same call on the same contents gives the same bits. */
 KERNIX_API size_t kx_attention_paged_ws(const kx_kv* c, int H, int n);
 KERNIX_API int kx_attention_paged(const kx_kv* c, int layer, const float* q, int ldq, int H, const int32_t* seqs, int n, int window,
                                   int sinks, float scale, float* ctx, int ldc, void* ws, size_t ws_bytes, int* status,
                                   void* stream);
 
 /* Attention of prompts with a sliding window whose first tokens stay visible (fp32 rows as kx_attention's, but heads that
- * share keys and values, ragged samples, any length). Sample b has q_len[b] <= Rq query rows b * Rq + i (ldq, H * dk
- * floats) and k_len[b] <= S key and value rows b * S + j (ldk, Hkv * dk; ldv, Hkv * dv); q_len, k_len: device words, NULL =
- * Rq, S. Its queries are the last tokens: query i is at position t = k_len - q_len + i and sees key j when j <= t and
- * (window <= 0 or j > t - window or j < sinks). ctx rows b * Rq + i (ldc, H * dv floats); a row that sees nothing (t < 0)
- * becomes 0, rows i >= q_len are left as they were; a sample whose lengths are out of range is reported
- * (KX_STATUS_BAD_REQUEST) and its Rq rows become NaN. Query head h reads key-value head h / (H / Hkv). scale 0 means
- * 1/sqrt(dk); |scale| < 2.3e38. dk, dv <= 128, H a multiple of Hkv. q, k, v must not overlap ctx or ws. ws: kx_attention_window_ws bytes
- * of device workspace (0: the arguments are invalid), 128-byte aligned, shared under kx_kv_ws's rules. Key and value
- * rows that no query of the sample sees do not affect results, not in their last bits either, whatever they hold; a row that
- * some queries see takes part in the roundings of its 64 neighbours. Accuracy is fp32's: products keep 2^-22 of their operands,
- * where an element of q (k or v) is not below 2^-16 of the largest in its row (in its 64 rows), or a weight not below 2^-16 of
- * the largest that its row has among those 64 keys; below that they keep 2^-38 of that largest. Blocks of 128 rows that see
- * NaN, infinities, magnitudes of 2^40 and more, rows of k or v 2^14 times above one of their neighbours, or 64 rows of v all
- * below 2^-40, are computed by plain fp32 code, 8 (128 keys a row) to 300 times slower (2500 keys). */
+ * share keys and values, ragged samples, any length). Sample b has q_len[b] <= Rq query rows b * Rq + i (ldq, H * dk floats)
+ * and k_len[b] <= S key and value rows b * S + j (ldk, Hkv * dk; ldv, Hkv * dv); q_len, k_len: device words, NULL = Rq, S.
+ * Its queries are the last tokens: query i is at position t = k_len - q_len + i and sees key j when j <= t and (window <= 0
+ * or j > t - window or j < sinks). ctx rows b * Rq + i (ldc, H * dv floats); a row that sees nothing (t < 0) becomes 0, rows
+ * i >= q_len are left as they were; a sample whose lengths are out of range is reported (KX_STATUS_BAD_REQUEST) and its Rq
+ * rows become NaN. Query head h reads key-value head h / (H / Hkv). scale 0 means 1/sqrt(dk); |scale| < 2.3e38. dk, dv <=
+ * 128, H a multiple of Hkv. q, k, v must not overlap ctx or ws. ws: kx_attention_window_ws bytes of device workspace (0: the
+ * arguments are invalid), 128-byte aligned, shared under kx_kv_ws's rules. Key and value rows that no query of the sample
+ * sees do not affect results, not in their last bits either, whatever they hold; a row that some queries see takes part in
+ * the roundings of its 64 neighbours. Accuracy is fp32's: products keep 2^-22 of their operands, where an element of q (k or
+ * v) is not below 2^-16 of the largest in its row (in its 64 rows), or a weight not below 2^-16 of the largest that its row
+ * has among those 64 keys; below that they keep 2^-38 of that largest. Blocks of 128 rows that see NaN, infinities,
+ * magnitudes of 2^40 and more, rows of k or v 2^14 times above one of their neighbours, or 64 rows of v all below 2^-40, are
+ * computed by plain fp32 code, 8 (128 keys a row) to 300 times slower (2500 keys). */
 KERNIX_API size_t kx_attention_window_ws(int B, int S, int Hkv, int dk, int dv);
 KERNIX_API int kx_attention_window(const float* q, int ldq, const float* k, int ldk, const float* v, int ldv, float* ctx, int ldc,
                                    int B, int Rq, int S, int H, int Hkv, int dk, int dv, const int32_t* q_len, const int32_t* k_len,
